@@ -591,6 +591,54 @@ typedef struct rs_adam_table {
 } rs_adam_table;
 int rs_adam_step(const rs_adam_table *t, double *hyper, int *step, int *done, int advance, void *stream);
 
+/* AdamW (decoupled weight decay) over a list of tensors, all fp32 or all bf16:
+ *   m += (g - m)(1 - b1);  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * -- the optimizer of the reference's segmentation loop (segmentation/tool/train.py), any number of tensors per call.
+ * The moments live in FLAT buffers in which tensor i starts at element at[i], a multiple of 256, and is followed by zeros up to the next
+ * multiple.  bits = 32: fp32 values.  bits = 8: one byte per element and, per 256 elements, one byte that holds the fp32 exponent
+ * field E of the block's largest finite |x|:
+ *   exp_avg     sign, 7 bits c: +-as_float(c << 20) * 2^(E - 14), c = 127: NaN;
+ *   exp_avg_sq  8 bits c:         as_float(c << 20) * 2^(E - 30), c = 255: infinity.
+ * An element is rounded up with the probability of the part that is cut off, by 16 bits of a hash of (seed, t, its block, its place in
+ * the block); a positive second moment keeps at least c = 1.  Zeroed buffers are the initial state.
+ * bf16 parameters: `low` (flat, like the moments) holds what the fp32 master has below the parameter: master bits =
+ * (parameter bits << 16) + low. */
+typedef struct rs_adamw_list {   /* HOST arrays of `count` entries; nothing is kept after the call */
+  int count;
+  void *const *p;                /* parameters, updated in place (contiguous, aligned to an element) */
+  const void *const *g;          /* gradients, of the parameters' type */
+  const long long *n;            /* elements, at least 1 */
+  const long long *at;           /* first element in the flat buffers */
+  const int *slot;               /* step[slot] counts the tensor's updates */
+} rs_adamw_list;
+typedef struct rs_adamw_args {
+  int bits, bf16;
+  void *exp_avg, *exp_avg_sq;
+  unsigned char *exp_avg_exponent, *exp_avg_sq_exponent;
+  short *low;
+  int *step, *done;              /* device: updates done per tensor, advanced by the call; an int that is 0 between calls */
+  const double *hyper_dev;       /* NULL: `hyper` counts; otherwise the same seven in device memory (a captured call follows them) */
+  double hyper[7];               /* lr, beta1, beta2, eps, weight_decay, ln beta1, ln beta2 */
+  const double *partial;         /* NULL, or npartial sums of squares: every g is multiplied by min(1, max_norm / (norm + 1e-6)) */
+  int npartial;
+  float max_norm;
+  float *norm;                   /* device: receives the norm */
+  unsigned seed;
+} rs_adamw_args;
+int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, void *stream);
+/* Sums of squares of the list's gradients, at most RS_GRAD_SQUARE_SUMS per 80 tensors, in an order that the sizes alone fix; *used
+ * (HOST) = their number, at most `room`.  l->p, at and slot are not used (p must not be NULL). */
+#define RS_GRAD_SQUARE_SUMS 512
+int rs_grad_square_sums(const rs_adamw_list *l, int bf16, double *partial, int room, int *used, void *stream);
+/* fp32 masters of the list's bf16 parameters, flat (what lies between tensors is left as it is) */
+int rs_adamw_masters(const rs_adamw_list *l, const short *low, float *out, void *stream);
+/* flat fp32 moments (n a multiple of 256) -> 8 bits, to nearest; 8 bits -> values in fp32 or bf16 (which holds them exactly, down to
+ * bf16's own smallest numbers) */
+int rs_adamw_pack(long long n, const float *m, const float *v, unsigned char *mc, unsigned char *vc, unsigned char *me,
+                  unsigned char *ve, void *stream);
+int rs_adamw_unpack(long long n, const unsigned char *mc, const unsigned char *vc, const unsigned char *me, const unsigned char *ve,
+                    int out_bf16, void *m, void *v, void *stream);
+
 /* Measurement aid (round 6): one-thread launch that stores the device's constant-rate wall clock (s_memrealtime) in *dst when it runs;
  * rs_timestamp_khz() = ticks per millisecond.  bench.py brackets a launch inside the step's replayed hipGraph with two of them (HIP
  * events cannot be recorded inside a replayed graph on this runtime).  Not used by the product path. */

@@ -9,7 +9,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("REPSURF_HIP_LIB") or os.path.join(_HERE, "lib", "librepsurf_hip.so")   # override: experiment builds only
-ABI_VERSION = 37
+ABI_VERSION = 38
 KNN_GRID_CELLS = 4096          # RS_KNN_GRID_CELLS of include/repsurf_hip.h
 
 c_int, c_float, c_void_p, c_ll = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
@@ -90,6 +90,11 @@ SIGNATURES = {
     "rs_furthestsampling_sectors": [c_int, c_int, P, P, P, P, P, P, P],
     "rs_take_int": [c_int, P, P, P, P],
     "rs_timestamp": [P, P],
+    "rs_adamw_step": [P, P, P],
+    "rs_grad_square_sums": [P, c_int, P, c_int, P, P],
+    "rs_adamw_masters": [P, P, P, P],
+    "rs_adamw_pack": [c_ll, P, P, P, P, P, P, P],
+    "rs_adamw_unpack": [c_ll, P, P, P, P, c_int, P, P, P],
     "rs_ballquery_grid_build": [c_int, c_int, c_float, P, P, P],
     "rs_ballquery_grid_query": [c_int, c_int, c_int, c_float, c_int, P, P, P, P, P],
 }
