@@ -8,7 +8,7 @@ LIBDIR := repsurf_amd/lib
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off \
             -fhip-fp32-correctly-rounded-divide-sqrt -munsafe-fp-atomics -Wall -Wno-unused-function
 SRCS := $(CSRC)/rs_lib.cpp $(CSRC)/fps.hip $(CSRC)/ballquery.hip $(CSRC)/knn_umbrella.hip $(CSRC)/knn_wide.hip \
-        $(CSRC)/group.hip $(CSRC)/interp.hip $(CSRC)/seg_geom.hip $(CSRC)/scene_knn.hip $(CSRC)/grid_knn.hip $(CSRC)/mlp.hip $(CSRC)/umbrella_mlp.hip $(CSRC)/umbrella_mfma.hip $(CSRC)/head.hip $(CSRC)/adam.hip $(CSRC)/adamw.hip
+        $(CSRC)/group.hip $(CSRC)/interp.hip $(CSRC)/seg_geom.hip $(CSRC)/scene_knn.hip $(CSRC)/grid_knn.hip $(CSRC)/mlp.hip $(CSRC)/umbrella_mlp.hip $(CSRC)/umbrella_mfma.hip $(CSRC)/head.hip $(CSRC)/adam.hip $(CSRC)/adamw.hip $(CSRC)/logits.hip
 OBJS := $(patsubst $(CSRC)/%,build/%.o,$(SRCS)) build/mlp_bf16.hip.o build/mlp_sb.hip.o build/mlp_split.hip.o
 
 # The geometry kernels run on a side stream BESIDE the network's MFMA kernels (graph.PipelinedStep / RaggedSegStep).  Packed-fp32 VALU
@@ -18,11 +18,11 @@ OBJS := $(patsubst $(CSRC)/%,build/%.o,$(SRCS)) build/mlp_bf16.hip.o build/mlp_s
 # profiles/r06/eager_beside_graph.txt).  Those translation
 # units -- and, at no measured cost (tools/slp_ab.sh), every other one without MFMA loops -- are compiled without the SLP and loop vectorizers; their
 # arithmetic is the same IEEE operations either way.
-GEOM_TUS := fps ballquery knn_umbrella knn_wide group interp seg_geom scene_knn grid_knn umbrella_mlp head adam adamw
+GEOM_TUS := fps ballquery knn_umbrella knn_wide group interp seg_geom scene_knn grid_knn umbrella_mlp head adam adamw logits
 $(foreach t,$(GEOM_TUS),$(eval build/$(t).hip.o: HIPFLAGS += -fno-slp-vectorize -fno-vectorize))
 # ... and these without packed-fp32 instructions at all
 NOPK := -Xclang -target-feature -Xclang -packed-fp32-ops
-build/adamw.hip.o: HIPFLAGS += $(NOPK)
+build/adamw.hip.o build/logits.hip.o: HIPFLAGS += $(NOPK)
 
 all: $(LIBDIR)/librepsurf_hip.so oracle
 

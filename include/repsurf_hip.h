@@ -639,6 +639,57 @@ int rs_adamw_pack(long long n, const float *m, const float *v, unsigned char *mc
 int rs_adamw_unpack(long long n, const unsigned char *mc, const unsigned char *vc, const unsigned char *me, const unsigned char *ve,
                     int out_bf16, void *m, void *v, void *stream);
 
+/* ---- objectives on log-probabilities of taken classes -----------------------------------------------
+ * Rows of logits (fp32, bf16 or fp16; `ld` elements apart, any alignment of an element) with a target class each; rows whose target is
+ * ignore_index are not read and count nowhere: log-probability 0, gradient 0.  offset (NULL or `sequences` int32): running row ends of
+ * packed sequences, like the clouds of a packed batch; rows behind the last end do not count either.  A target outside [0, classes)
+ * makes its row's log-probability, loss and gradient NaN and adds 1 to *bad_labels (device int, may be NULL).  Row statistics are
+ * collected in fp64 and nothing depends on an order of atomics. */
+typedef struct rs_logits {
+  const void *logits;
+  long long rows, ld;
+  int classes, type;             /* type: 0 fp32, 1 bf16, 2 fp16 */
+  const long long *target;
+  long long ignore_index;
+  const int *offset;
+  int sequences;
+  int *bad_labels;
+} rs_logits;
+/* log softmax(logits)[target]: logp (fp32) and / or logp64; stat (rows, 2), may be NULL: what a backward pass needs */
+int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64, float *stat, void *stream);
+/* dlogits (rows, classes; contiguous, of the logits' type) = c * ([j = target] - softmax_j), c = coef[row] -- with offsets coef[sequence] --
+ * times *gout (NULL: 1).  skip_unit: nothing is done where *gout is 1 (dlogits holds that result already). */
+int rs_token_logprobs_backward(const rs_logits *l, const float *stat, const float *coef, const float *gout, int skip_unit, void *dlogits,
+                               void *stream);
+/* per sequence: the sum of its rows' log-probabilities, or (average) their mean over the rows that count: sums (fp64), out (fp32), each
+ * (fp32) = the factor of a row in it; any of the three may be NULL */
+int rs_sequence_sums(const rs_logits *l, const double *logp64, int average, double *sums, float *out, float *each, void *stream);
+/* paired log ratios: sequence i is preferred to sequence pairs + i; r = beta (sums - ref), h = r_i - r_(pairs + i),
+ * loss = mean of -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h); rewards (2 pairs) = r; coef (2 pairs) = d loss / d (a row's
+ * log-probability) */
+int rs_preference_pairs(int pairs, const double *sums, const float *each, const float *ref, double beta, double smoothing, float *loss,
+                        float *rewards, float *coef, void *stream);
+/* clipped policy loss: per row that counts, with x = log p(target), r = exp(x - old_logp), A = advantages (per row, or per sequence):
+ *   -min(r A, clamp(r, low, high) A) + kl_coef (exp(d) - 1 - d),  d = ref_logp - x (ref_logp NULL: without that term)
+ * averaged over the rows that count (token_mean), or over every sequence's rows and then over the sequences (one without any adds 0).
+ * stats (2) = mean of exp(d) - 1 - d, share of rows whose ratio was cut off (both weighted like the loss).  With dlogits: the
+ * gradient, and coef (rows) / stat (rows, 2) for rs_token_logprobs_backward. */
+typedef struct rs_policy {
+  const float *old_logp, *advantages, *ref_logp;
+  int advantages_per_sequence, token_mean;
+  double low, high, kl_coef;
+  int *counts;                   /* scratch: RS_POLICY_COUNTS * (token_mean ? 1 : sequences) ints are enough */
+  int counts_room;
+  double *partial;               /* scratch: RS_POLICY_PARTIAL doubles are enough */
+  int partial_room;
+  float *loss, *stats, *logp;    /* logp (rows) may be NULL */
+  void *dlogits;
+  float *coef, *stat;
+} rs_policy;
+#define RS_POLICY_COUNTS 64
+#define RS_POLICY_PARTIAL 6144
+int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stream);
+
 /* Measurement aid (round 6): one-thread launch that stores the device's constant-rate wall clock (s_memrealtime) in *dst when it runs;
  * rs_timestamp_khz() = ticks per millisecond.  bench.py brackets a launch inside the step's replayed hipGraph with two of them (HIP
  * events cannot be recorded inside a replayed graph on this runtime).  Not used by the product path. */
