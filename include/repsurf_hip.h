@@ -655,8 +655,11 @@ typedef struct rs_logits {
   int sequences;
   int *bad_labels;
 } rs_logits;
-/* log softmax(logits)[target]: logp (fp32) and / or logp64; stat (rows, 2), may be NULL: what a backward pass needs */
-int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64, float *stat, void *stream);
+/* log softmax(logits)[target]: logp (fp32) and / or logp64; stat (rows, 2), may be NULL: what a backward pass needs.  scratch: NULL, or for
+ * at most RS_LOGITS_FEW_ROWS rows 12 * RS_LOGITS_PARTS bytes each (aligned to 8): a few long rows are then cut over many workgroups */
+#define RS_LOGITS_FEW_ROWS 256
+#define RS_LOGITS_PARTS 64
+int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64, float *stat, void *scratch, void *stream);
 /* dlogits (rows, classes; contiguous, of the logits' type) = c * ([j = target] - softmax_j), c = coef[row] -- with offsets coef[sequence] --
  * times *gout (NULL: 1).  skip_unit: nothing is done where *gout is 1 (dlogits holds that result already). */
 int rs_token_logprobs_backward(const rs_logits *l, const float *stat, const float *coef, const float *gout, int skip_unit, void *dlogits,
@@ -680,11 +683,12 @@ typedef struct rs_policy {
   double low, high, kl_coef;
   int *counts;                   /* scratch: RS_POLICY_COUNTS * (token_mean ? 1 : sequences) ints are enough */
   int counts_room;
-  double *partial;               /* scratch: RS_POLICY_PARTIAL doubles are enough */
+  double *partial;               /* scratch: RS_POLICY_PARTIAL doubles */
   int partial_room;
   float *loss, *stats, *logp;    /* logp (rows) may be NULL */
   void *dlogits;
   float *coef, *stat;
+  void *scratch;                 /* as in rs_token_logprobs */
 } rs_policy;
 #define RS_POLICY_COUNTS 64
 #define RS_POLICY_PARTIAL 6144

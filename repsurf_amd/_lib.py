@@ -95,7 +95,7 @@ SIGNATURES = {
     "rs_adamw_masters": [P, P, P, P],
     "rs_adamw_pack": [c_ll, P, P, P, P, P, P, P],
     "rs_adamw_unpack": [c_ll, P, P, P, P, c_int, P, P, P],
-    "rs_token_logprobs": [P, P, P, P, P],
+    "rs_token_logprobs": [P, P, P, P, P, P],
     "rs_token_logprobs_backward": [P, P, P, P, c_int, P, P],
     "rs_sequence_sums": [P, P, c_int, P, P, P, P],
     "rs_preference_pairs": [c_int, P, P, P, ctypes.c_double, ctypes.c_double, P, P, P, P],

@@ -32,48 +32,92 @@ struct Policy {
   double *partial;            // per workgroup: loss, KL, cut-off rows
 };
 
-template <typename T> __device__ __forceinline__ float lg_wide(T x) { return (float)x; }
-
 constexpr int LG_VEC = 8;
 template <typename T> struct Vec { T x[LG_VEC]; };
 // 8 consecutive logits, aligned to one of them: global loads and stores of this device need no more
 template <typename T>
-__device__ __forceinline__ void lg_load(const T *p, int left, float *x) {
-  if (left >= LG_VEC) {
-    Vec<T> v;
-    __builtin_memcpy(&v, p, sizeof(v));
+__device__ __forceinline__ Vec<T> lg_load(const T *p, int left) {
+  Vec<T> v;
+  if (left >= LG_VEC) __builtin_memcpy(&v, p, sizeof(v));
+  else {
 #pragma unroll
-    for (int i = 0; i < LG_VEC; ++i) x[i] = lg_wide(v.x[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < LG_VEC; ++i) x[i] = i < left ? lg_wide(p[i]) : -INFINITY;
+    for (int i = 0; i < LG_VEC; ++i) v.x[i] = i < left ? p[i] : (T)-INFINITY;
   }
+  return v;
 }
 template <typename T>
 __device__ __forceinline__ void lg_store(T *p, int left, const float *x) {
-  if (left >= LG_VEC) {
-    Vec<T> v;
+  Vec<T> v;
 #pragma unroll
-    for (int i = 0; i < LG_VEC; ++i) v.x[i] = (T)x[i];
-    __builtin_memcpy(p, &v, sizeof(v));
-  } else {
+  for (int i = 0; i < LG_VEC; ++i) v.x[i] = (T)x[i];
+  if (left >= LG_VEC) __builtin_memcpy(p, &v, sizeof(v));
+  else {
 #pragma unroll
-    for (int i = 0; i < LG_VEC; ++i) if (i < left) p[i] = (T)x[i];
+    for (int i = 0; i < LG_VEC; ++i) if (i < left) p[i] = v.x[i];
   }
 }
+template <typename T>
+__device__ __forceinline__ float lg_top(const Vec<T> &v, float m) {
+#pragma unroll
+  for (int i = 0; i < LG_VEC; ++i) m = fmaxf(m, (float)v.x[i]);
+  return m;
+}
 
-__device__ __forceinline__ float lg_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+// exp(x).  log2 e in two parts: its fp32 rounding alone would shift every row's sum the same way (1.3e-8 |x|), and a sequence's log-probability
+// adds thousands of rows
+__device__ __forceinline__ float lg_exp(float x) {
+  return __builtin_amdgcn_exp2f(rs_fma(x, 1.44269502162933349609f, x * 1.92596299112661746887e-8f));
+}
+template <typename T>
+__device__ __forceinline__ double lg_sum(const Vec<T> &v, float base) {
+  float e[LG_VEC];
+#pragma unroll
+  for (int i = 0; i < LG_VEC; ++i) e[i] = lg_exp((float)v.x[i] - base);
+  return (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
+}
+// c ([j = y] - exp(z_j - base) inv), scale = -c inv; j: the index of v's first logit
+template <typename T>
+__device__ __forceinline__ void lg_gradient(T *p, int left, const Vec<T> &v, float base, float scale, float c, int j, int y) {
+  float g[LG_VEC];
+#pragma unroll
+  for (int i = 0; i < LG_VEC; ++i) g[i] = lg_exp((float)v.x[i] - base) * scale;
+  if (((j ^ y) & ~(LG_VEC - 1)) == 0) {
+#pragma unroll
+    for (int i = 0; i < LG_VEC; ++i) g[i] += j + i == y ? c : 0.f;
+  }
+  lg_store(p, left, g);
+}
+template <typename T>
+__device__ __forceinline__ void lg_fill(T *p, int left, float x) {
+  float g[LG_VEC];
+#pragma unroll
+  for (int i = 0; i < LG_VEC; ++i) g[i] = x;
+  lg_store(p, left, g);
+}
+// The compiler must not keep what it formed of v (conversions, exponentials) past this point: in fp32 that is twice the registers of a
+// row in 16 bits, and a kernel that holds rows would spill.
+template <typename T>
+__device__ __forceinline__ void lg_forget(Vec<T> &v) {
+  unsigned w[sizeof(v) / 4];
+  __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(v) / 4); ++i) asm volatile("" : "+v"(w[i]));
+  __builtin_memcpy(&v, w, sizeof(v));
+}
 // the value that exponents are taken against: of a row that holds nothing but -infinity, 0 (exp(-inf - 0) = 0, and 0 / 0 follows)
 __device__ __forceinline__ float lg_base(float m) { return m == -INFINITY ? 0.f : m; }
 
-__device__ __forceinline__ float lg_wave_max(float x) {
+// over LANES neighbouring lanes, the result in each of them
+template <int LANES>
+__device__ __forceinline__ float lg_lanes_max(float x) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  for (int o = LANES / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
   return x;
 }
-__device__ __forceinline__ double lg_wave_sum(double x) {
+template <int LANES>
+__device__ __forceinline__ double lg_lanes_sum(double x) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
 
@@ -87,180 +131,368 @@ __device__ __forceinline__ int lg_owner(const int *offset, int sequences, long l
   return lo;
 }
 
-enum { LG_LOGP = 0, LG_POLICY = 1 };
+// exp, log and exp(d) - 1 - d in fp64, in a chain of few registers: they run while a row waits in the others.  exp(x) = 2^k exp(r), |r| <= ln 2 / 2,
+// as its Taylor sum to r^13 / 13! (r^14 / 14!: 4e-18); log s = y + log(s exp(-y)) from fp32's y, whose rest is below 1e-6.
+__device__ __forceinline__ double lg_taylor(double r, double from) {      // sum of r^i / (i + 2)!, the exponential without its first two terms over r^2
+  double t = 1.0 / 6227020800.0;
+  t = fma(t, r, 1.0 / 479001600.0); t = fma(t, r, 1.0 / 39916800.0); t = fma(t, r, 1.0 / 3628800.0); t = fma(t, r, 1.0 / 362880.0);
+  t = fma(t, r, 1.0 / 40320.0); t = fma(t, r, 1.0 / 5040.0); t = fma(t, r, 1.0 / 720.0); t = fma(t, r, 1.0 / 120.0); t = fma(t, r, 1.0 / 24.0);
+  t = fma(t, r, 1.0 / 6.0);
+  return fma(t, r, from);
+}
+__device__ __forceinline__ double lg_exp64(double x) {
+  const double lim = fmin(fmax(x, -1100.0), 1100.0);                  // (infinite arguments; not-a-numbers are put back below)
+  const double k = rint(lim * 1.4426950408889634074);
+  const double r = fma(-k, 2.3190468138462995584e-17, fma(-k, 0.69314718055994528623, lim));
+  const double e = fma(fma(lg_taylor(r, 0.5), r, 1.0), r, 1.0);
+  return x != x ? x : ldexp(e, (int)k);
+}
+__device__ __forceinline__ double lg_log64(double s) {                  // of a sum: at least 1, or infinite, or no number
+  const double y = (double)(__builtin_amdgcn_logf((float)s) * 0.69314718055994530942f);
+  const double q = fma(s, lg_exp64(-y), -1.0);
+  return s < INFINITY ? y + fma(-0.5 * q, q, q) : s;
+}
+__device__ __forceinline__ double lg_rest(double d) {                    // exp(d) - 1 - d
+  return fabs(d) <= 0.35 ? d * d * lg_taylor(d, 0.5) : lg_exp64(d) - 1.0 - d;
+}
 
 // d loss / d log p(y) of the policy loss for one row, and its three contributions
-__device__ __forceinline__ double lg_policy(const Policy &P, double w, double logp, double old, double a, bool has_ref, double ref, double *add) {
-  const double r = exp(logp - old);
+__device__ __forceinline__ double lg_policy(const Policy &P, double w, double logp, double old, double a, double ref, double *add) {
+  const double r = lg_exp64(logp - old);
   const bool cut = a >= 0.0 ? r > P.hi : r < P.lo;             // the cut-off ratio is the smaller term: no gradient through it
   double each = -(cut ? (a >= 0.0 ? P.hi : P.lo) : r) * a, c = cut ? 0.0 : -a * r;
   if (r != r || a != a) each = c = r + a;
-  if (has_ref) {
-    const double d = ref - logp, e = expm1(d);                 // exp(d) - 1 - d: not negative, and its mean over the policy's own draws is the KL
-    each += P.kl * (e - d);
-    c -= P.kl * e;
-    add[1] += w * (e - d);
+  if (P.ref) {
+    const double d = ref - logp, e = lg_rest(d);               // not negative, and its mean over the policy's own draws is the KL
+    each += P.kl * e;
+    c -= P.kl * (e + d);
+    add[1] += w * e;
   }
   add[0] += w * each;
   add[2] += cut ? w : 0.0;
   return w * c;
 }
+__device__ __forceinline__ double lg_weight(const Rows &R, const Policy &P, int owner) {
+  int n = 0;
+  const int first = P.token_mean ? 0 : owner * P.splits;
+  for (int k = 0; k < P.splits; ++k) n += P.counts[first + k];
+  return 1.0 / (double)n / (P.token_mean ? 1.0 : (double)R.sequences);
+}
 
-// One team of WAVES waves per row, `4 / WAVES` (at least 1) teams per workgroup, rows taken in turn by the grid's teams.
-//   LG_LOGP:   logp / logp64 / stat of every row
-//   LG_POLICY: the policy loss's contributions, logp, and -- with dlogits -- the gradient and coef / stat for a later backward pass
-template <typename T, int MODE, int WAVES>
-__global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
-rows_kernel(Rows R, Policy P, float *__restrict__ logp_out, double *__restrict__ logp64, float2 *__restrict__ stat, T *__restrict__ dz) {
-  constexpr int TEAMS = WAVES < 4 ? 4 / WAVES : 1;
-  constexpr int LANES = WAVES * 64;
-  __shared__ float red_m[WAVES];
-  __shared__ double red_s[WAVES];
-  __shared__ float row_c;
-  __shared__ double sums[3][TEAMS];
-  static_assert(WAVES == 1 || TEAMS == 1, "a team of several waves is the workgroup: its barriers are the workgroup's");
-  const int team = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES, wave = lane >> 6;
-  double add[3] = {0.0, 0.0, 0.0};
-  const int V = R.classes;
-  for (long long row = (long long)blockIdx.x * TEAMS + team; row < R.rows; row += (long long)gridDim.x * TEAMS) {
-    const T *__restrict__ z = (const T *)R.z + row * R.ld;
-    const long long y = R.target[row];
-    int owner = 0;
-    if (R.offset) owner = lg_owner(R.offset, R.sequences, row);
-    const bool counts = y != R.ignore && (!R.offset || owner < R.sequences);
-    const bool bad = counts && (y < 0 || y >= V);
-    if (!counts || bad) {               // nothing of the row is read
-      const float fill = bad ? __uint_as_float(0x7FC00000u) : 0.f;
-      if (lane == 0) {
-        if (logp_out) logp_out[row] = fill;
-        if (logp64) logp64[row] = (double)fill;
-        if (stat) stat[row] = make_float2(fill, 0.f);
-        if (bad && R.bad) atomicAdd(R.bad, 1);
-        if (MODE == LG_POLICY) {
-          if (P.coef) P.coef[row] = fill;
-          if (bad) { add[0] += (double)fill; add[1] += (double)fill; add[2] += (double)fill; }
-        }
-      }
-      if (MODE == LG_POLICY && dz) {
-        float x[LG_VEC];
-#pragma unroll
-        for (int i = 0; i < LG_VEC; ++i) x[i] = fill;
-        for (int j = lane * LG_VEC; j < V; j += LANES * LG_VEC) lg_store(dz + row * V + j, V - j, x);
-      }
-      continue;
-    }
-    float m = -INFINITY;
-    double s = 0.0;
-    for (int j = lane * LG_VEC; j < V; j += LANES * LG_VEC) {
-      float x[LG_VEC];
-      lg_load(z + j, V - j, x);
-      float top = x[0];
-#pragma unroll
-      for (int i = 1; i < LG_VEC; ++i) top = fmaxf(top, x[i]);
-      if (top > m) { s *= (double)lg_exp(m - top); m = top; }       // (m = -inf at first: s is 0)
-      const float base = lg_base(m);
-      float e = 0.f;
-#pragma unroll
-      for (int i = 0; i < LG_VEC; ++i) e += lg_exp(x[i] - base);
-      s += (double)e;
-    }
-    float M = lg_wave_max(m);
-    if (WAVES > 1) {
-      __syncthreads();                  // (the row before this one is done with the scratch)
-      if ((lane & 63) == 0) red_m[wave] = M;
-      __syncthreads();
-      M = red_m[0];
-      for (int k = 1; k < WAVES; ++k) M = fmaxf(M, red_m[k]);
-    }
-    s = lg_wave_sum(m == -INFINITY ? s : s * (double)lg_exp(m - lg_base(M)));
-    if (WAVES > 1) {
-      if ((lane & 63) == 0) red_s[wave] = s;
-      __syncthreads();
-      s = 0.0;
-      for (int k = 0; k < WAVES; ++k) s += red_s[k];
-    }
-    const float inv = (float)(1.0 / s);
-    float c = 0.f;
-    if (lane == 0) {
-      const double lp = (double)lg_wide(z[y]) - (double)M - log(s);
-      if (logp_out) logp_out[row] = (float)lp;
-      if (logp64) logp64[row] = lp;
-      if (stat) stat[row] = make_float2(M, inv);
-      if (MODE == LG_POLICY) {
-        int n = 0;
-        const int first = P.token_mean ? 0 : owner * P.splits;
-        for (int k = 0; k < P.splits; ++k) n += P.counts[first + k];
-        const double w = 1.0 / (double)n / (P.token_mean ? 1.0 : (double)R.sequences);
-        c = (float)lg_policy(P, w, lp, (double)P.old_logp[row], (double)P.adv[P.adv_per_sequence ? (long long)owner : row], P.ref != nullptr,
-                             P.ref ? (double)P.ref[row] : 0.0, add);
-        if (P.coef) P.coef[row] = c;
-      }
-    }
-    if (MODE == LG_POLICY && dz) {
-      if (WAVES > 1) {
-        if (lane == 0) row_c = c;
-        __syncthreads();
-        c = row_c;
-      } else c = __shfl(c, 0);
-      const float base = lg_base(M), scale = -c * inv;
-      for (int j = lane * LG_VEC; j < V; j += LANES * LG_VEC) {
-        float x[LG_VEC];
-        lg_load(z + j, V - j, x);
-#pragma unroll
-        for (int i = 0; i < LG_VEC; ++i) x[i] = rs_fma(lg_exp(x[i] - base), scale, j + i == (int)y ? c : 0.f);
-        lg_store(dz + row * V + j, V - j, x);
-      }
+enum { LG_LOGP = 0, LG_POLICY = 1, LG_BACK = 2 };
+
+// what a row is, before any of its logits is read
+struct Row {
+  long long at, y;
+  int owner;
+  bool counts, bad;
+};
+__device__ __forceinline__ Row lg_row(const Rows &R, long long row) {
+  Row w;
+  w.at = row;
+  w.y = R.target[row];
+  w.owner = R.offset ? lg_owner(R.offset, R.sequences, row) : 0;
+  w.counts = w.y != R.ignore && (!R.offset || w.owner < R.sequences);
+  w.bad = w.counts && (w.y < 0 || w.y >= R.classes);
+  return w;
+}
+
+struct Outs {                 // what a kernel writes of a row; null: not wanted
+  float *logp;
+  double *logp64;
+  float2 *stat;               // M, 1 / s
+  void *dz;
+  const float *coef, *up;     // LG_BACK: coefficients of rows (of sequences with offsets), and a factor for all of them
+  int skip_unit;
+};
+
+// one that does not count, or whose target is no class: 0, or not a number; none of its logits is read
+__device__ __forceinline__ float lg_void(const Rows &R, const Policy &P, const Outs &O, const Row &w, bool first, int policy, double *add) {
+  const float fill = w.bad ? __uint_as_float(0x7FC00000u) : 0.f;
+  if (first) {
+    if (O.logp) O.logp[w.at] = fill;
+    if (O.logp64) O.logp64[w.at] = (double)fill;
+    if (O.stat) O.stat[w.at] = make_float2(fill, 0.f);
+    if (w.bad && R.bad) atomicAdd(R.bad, 1);
+    if (policy) {
+      if (P.coef) P.coef[w.at] = fill;
+      if (w.bad) { add[0] += (double)fill; add[1] += (double)fill; add[2] += (double)fill; }
     }
   }
-  if (MODE == LG_POLICY) {
-    if (lane == 0) { sums[0][team] = add[0]; sums[1][team] = add[1]; sums[2][team] = add[2]; }
-    __syncthreads();
-    if (threadIdx.x == 0)
-      for (int k = 0; k < 3; ++k) {
-        double t = 0.0;
-        for (int i = 0; i < TEAMS; ++i) t += sums[k][i];
-        P.partial[(long long)blockIdx.x * 3 + k] = t;
-      }
+  return fill;
+}
+// what follows from a row's M and s.  All lanes of a team compute it: it costs a wave the same as one lane does.
+template <typename T>
+__device__ __forceinline__ float lg_finish(const Rows &R, const Policy &P, const Outs &O, const Row &w, float zy, float M, double s, bool first, int policy,
+                                           double *add) {
+  const double lp = (double)zy - (double)M - lg_log64(s);
+  float c = 0.f;
+  double mine[3] = {0.0, 0.0, 0.0};
+  if (policy)
+    c = (float)lg_policy(P, lg_weight(R, P, w.owner), lp, (double)P.old_logp[w.at], (double)P.adv[P.adv_per_sequence ? (long long)w.owner : w.at],
+                         P.ref ? (double)P.ref[w.at] : 0.0, mine);
+  if (first) {
+    if (O.logp) O.logp[w.at] = (float)lp;
+    if (O.logp64) O.logp64[w.at] = lp;
+    if (O.stat) O.stat[w.at] = make_float2(M, 1.f / (float)s);
+    if (policy) {
+      if (P.coef) P.coef[w.at] = c;
+      add[0] += mine[0]; add[1] += mine[1]; add[2] += mine[2];
+    }
+  }
+  return c;
+}
+
+// the policy loss's sums of a workgroup, in the order of its threads
+template <int THREADS>
+__device__ __forceinline__ void lg_partial(const Policy &P, const double *add, int block) {
+  __shared__ double red[3][THREADS / 64];
+  for (int k = 0; k < 3; ++k) {
+    const double t = lg_lanes_sum<64>(add[k]);
+    if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = t;
+  }
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    double t = 0.0;
+    for (int i = 0; i < THREADS / 64; ++i) t += red[threadIdx.x][i];
+    P.partial[(long long)block * 3 + threadIdx.x] = t;
   }
 }
 
-// dz = c ([j = y] - exp(z_j - M) / s) with the rows' saved M and 1 / s; c = coef of the row (or of its sequence) times *gout
-template <typename T, int WAVES>
-__global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
-rows_backward_kernel(Rows R, const float2 *__restrict__ stat, const float *__restrict__ coef, const float *__restrict__ gout, int skip_unit,
-                     T *__restrict__ dz) {
-  constexpr int TEAMS = WAVES < 4 ? 4 / WAVES : 1;
-  constexpr int LANES = WAVES * 64;
-  const float up = gout ? *gout : 1.f;
-  if (skip_unit && up == 1.f) return;
-  const int team = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES;
-  const int V = R.classes;
-  for (long long row = (long long)blockIdx.x * TEAMS + team; row < R.rows; row += (long long)gridDim.x * TEAMS) {
+// Rows of up to 2048 classes: LANES neighbouring lanes hold a row in NV vectors of 8 per lane; one read, one write.  With 13 classes a wave
+// works on 32 rows at once, so the fp64 steps of a row cost a 32nd of a wave's.
+template <typename T, int MODE, int LANES, int NV>
+__global__ void __launch_bounds__(256)
+short_kernel(Rows R, Policy P, Outs O) {
+  constexpr int TEAMS = 256 / LANES;
+  const float up = MODE == LG_BACK && O.up ? *O.up : 1.f;
+  if (MODE == LG_BACK && O.skip_unit && up == 1.f) return;
+  const int team = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES, V = R.classes;
+  double add[3] = {0.0, 0.0, 0.0};
+  for (long long first = (long long)blockIdx.x * TEAMS; first < R.rows; first += (long long)gridDim.x * TEAMS) {
+    const long long row = first + team;
+    const bool live = row < R.rows;                            // (all lanes take part in the exchanges below)
+    Row w{row, 0, 0, false, false};
+    if (live) w = lg_row(R, row);
+    const bool in = w.counts && !w.bad;
     const T *__restrict__ z = (const T *)R.z + row * R.ld;
-    const long long y = R.target[row];
-    int owner = 0;
-    if (R.offset) owner = lg_owner(R.offset, R.sequences, row);
-    const bool counts = y != R.ignore && (!R.offset || owner < R.sequences);
-    float c = 0.f;
-    if (counts) c = coef[R.offset ? (long long)owner : row] * up;
-    if (counts && (y < 0 || y >= V)) c = __uint_as_float(0x7FC00000u);
-    if (!counts || c == 0.f || c != c) {
-      float x[LG_VEC];
+    T *__restrict__ dz = O.dz ? (T *)O.dz + row * V : nullptr;
+    Vec<T> v[NV];
+    float c = 0.f, M = -INFINITY, inv = 0.f;
 #pragma unroll
-      for (int i = 0; i < LG_VEC; ++i) x[i] = c;
-      for (int j = lane * LG_VEC; j < V; j += LANES * LG_VEC) lg_store(dz + row * V + j, V - j, x);
-      continue;
+    for (int k = 0; k < NV; ++k) {
+      const int j = (k * LANES + lane) * LG_VEC;
+      v[k] = lg_load(z + j, in ? V - j : 0);
     }
-    const float2 st = stat[row];
-    const float base = lg_base(st.x), scale = -c * st.y;
-    for (int j = lane * LG_VEC; j < V; j += LANES * LG_VEC) {
-      float x[LG_VEC];
-      lg_load(z + j, V - j, x);
+    if (MODE == LG_BACK) {
+      if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w.owner : row] * up;
+      if (in) { const float2 st = O.stat[row]; M = st.x; inv = st.y; }
+    } else {
+      const float zy = in ? (float)z[w.y] : 0.f;
 #pragma unroll
-      for (int i = 0; i < LG_VEC; ++i) x[i] = rs_fma(lg_exp(x[i] - base), scale, j + i == (int)y ? c : 0.f);
-      lg_store(dz + row * V + j, V - j, x);
+      for (int k = 0; k < NV; ++k) { M = lg_top(v[k], M); if (NV > 1) lg_forget(v[k]); }
+      M = lg_lanes_max<LANES>(M);
+      double s = 0.0;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) { s += lg_sum(v[k], lg_base(M)); if (NV > 1) lg_forget(v[k]); }
+      s = lg_lanes_sum<LANES>(s);
+      if (in) c = lg_finish<T>(R, P, O, w, zy, M, s, lane == 0, MODE == LG_POLICY, add);
+      else if (live) c = lg_void(R, P, O, w, lane == 0, MODE == LG_POLICY, add);
+      inv = 1.f / (float)s;
+    }
+    if (MODE != LG_LOGP && dz && live) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int j = (k * LANES + lane) * LG_VEC;
+        if (j >= V) continue;
+        if (in && c == c) lg_gradient(dz + j, V - j, v[k], lg_base(M), -c * inv, c, j, (int)w.y);
+        else lg_fill(dz + j, V - j, c);
+      }
     }
   }
+  if (MODE == LG_POLICY) lg_partial<256>(P, add, (int)blockIdx.x);
+}
+
+// Long rows, one workgroup each, LDS for what its waves tell each other.  HELD (the policy loss): the row stays in registers between its
+// sum and its gradient, NV vectors of 8 per thread.  Otherwise chunks of NV vectors are taken in turn: their loads are all in flight
+// before the first is used, and the running maximum is corrected once per chunk.
+template <typename T, int MODE, int THREADS, int NV, bool HELD>
+__global__ void __launch_bounds__(THREADS)
+long_kernel(Rows R, Policy P, Outs O) {
+  constexpr int W = THREADS / 64;
+  __shared__ float red_m[2][W];
+  __shared__ double red_s[2][W];
+  __shared__ float red_c[2];
+  const int tid = (int)threadIdx.x, wave = tid >> 6, V = R.classes;
+  double add[3] = {0.0, 0.0, 0.0};
+  int turn = 0;                       // scratch of two rows in turn: a row's last reader is a barrier ahead of the next but one's writer
+  for (long long row = blockIdx.x; row < R.rows; row += gridDim.x) {
+    const Row w = lg_row(R, row);
+    const T *__restrict__ z = (const T *)R.z + row * R.ld;
+    T *__restrict__ dz = O.dz ? (T *)O.dz + row * V : nullptr;
+    if (!w.counts || w.bad) {
+      const float fill = lg_void(R, P, O, w, tid == 0, MODE == LG_POLICY, add);
+      if (MODE == LG_POLICY && dz)
+        for (int j = tid * LG_VEC; j < V; j += THREADS * LG_VEC) lg_fill(dz + j, V - j, fill);
+      continue;
+    }
+    turn ^= 1;
+    Vec<T> v[NV];
+    float m = -INFINITY, M;
+    double s = 0.0;
+    const float zy = (float)z[w.y];
+    if (HELD) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) v[k] = lg_load(z + (k * THREADS + tid) * LG_VEC, V - (k * THREADS + tid) * LG_VEC);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) { m = lg_top(v[k], m); lg_forget(v[k]); }
+    } else {
+      for (int j0 = 0; j0 < V; j0 += THREADS * LG_VEC * NV) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) { const int j = j0 + (k * THREADS + tid) * LG_VEC; v[k] = lg_load(z + (j < V ? j : 0), V - j); }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) top = lg_top(v[k], top);
+        if (top > m) { s *= (double)lg_exp(m - top); m = top; }          // (m = -inf at first: s is 0)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) s += lg_sum(v[k], lg_base(m));
+      }
+    }
+    M = lg_lanes_max<64>(m);
+    if ((tid & 63) == 0) red_m[turn][wave] = M;
+    __syncthreads();
+    M = red_m[turn][0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) M = fmaxf(M, red_m[turn][k]);
+    float base = lg_base(M);
+    if (HELD) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) { s += lg_sum(v[k], base); lg_forget(v[k]); }
+    } else if (m != -INFINITY) s *= (double)lg_exp(m - base);
+    s = lg_lanes_sum<64>(s);
+    if ((tid & 63) == 0) red_s[turn][wave] = s;
+    __syncthreads();
+    s = red_s[turn][0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) s += red_s[turn][k];
+    float c = 0.f;
+    if (wave == 0) {
+      c = lg_finish<T>(R, P, O, w, zy, M, s, tid == 0, MODE == LG_POLICY, add);
+      if (tid == 0) red_c[turn] = c;
+    }
+    if (MODE == LG_POLICY && dz) {
+      __syncthreads();
+      c = red_c[turn];
+      const float scale = -c * (1.f / (float)s);
+      if (HELD) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int j = (k * THREADS + tid) * LG_VEC;
+          if (j >= V) continue;
+          if (c == c) lg_gradient(dz + j, V - j, v[k], base, scale, c, j, (int)w.y);
+          else lg_fill(dz + j, V - j, c);
+        }
+      } else {
+        for (int j = tid * LG_VEC; j < V; j += THREADS * LG_VEC) {
+          if (c == c) lg_gradient(dz + j, V - j, lg_load(z + j, V - j), base, scale, c, j, (int)w.y);
+          else lg_fill(dz + j, V - j, c);
+        }
+      }
+    }
+  }
+  if (MODE == LG_POLICY) lg_partial<THREADS>(P, add, (int)blockIdx.x);
+}
+
+// backward pass of long rows: a workgroup takes 256 * 8 * NV logits of a row at a time, whatever row they are of
+template <typename T, int NV>
+__global__ void __launch_bounds__(256)
+long_back_kernel(Rows R, Outs O, int parts) {
+  const float up = O.up ? *O.up : 1.f;
+  if (O.skip_unit && up == 1.f) return;
+  const int tid = (int)threadIdx.x, V = R.classes;
+  const long long all = R.rows * parts;
+  for (long long b = blockIdx.x; b < all; b += gridDim.x) {
+    const long long row = b / parts;
+    const int j0 = (int)(b - row * parts) * (256 * LG_VEC * NV);
+    const Row w = lg_row(R, row);
+    const T *__restrict__ z = (const T *)R.z + row * R.ld;
+    T *__restrict__ dz = (T *)O.dz + row * V;
+    float c = 0.f;
+    if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w.owner : row] * up;
+    if (c == 0.f || c != c) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; if (j < V) lg_fill(dz + j, V - j, c); }
+      continue;
+    }
+    const float2 st = O.stat[row];
+    Vec<T> v[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; v[k] = lg_load(z + (j < V ? j : 0), V - j); }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int j = j0 + (k * 256 + tid) * LG_VEC;
+      if (j < V) lg_gradient(dz + j, V - j, v[k], lg_base(st.x), -c * st.y, c, j, (int)w.y);
+    }
+  }
+}
+
+// Few long rows: a row in `parts` pieces, (M, s) of each ...
+template <typename T, int NV>
+__global__ void __launch_bounds__(256)
+part_kernel(Rows R, int parts, int piece, float *__restrict__ part_m, double *__restrict__ part_s) {
+  __shared__ float red_m[4];
+  __shared__ double red_s[4];
+  const int tid = (int)threadIdx.x;
+  const long long row = blockIdx.y;
+  const Row w = lg_row(R, row);
+  if (!w.counts || w.bad) return;
+  const int from = (int)blockIdx.x * piece, to = min(R.classes, from + piece);
+  const T *__restrict__ z = (const T *)R.z + row * R.ld;
+  float m = -INFINITY;
+  double s = 0.0;
+  for (int j0 = from; j0 < to; j0 += 256 * LG_VEC * NV) {
+    Vec<T> v[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; v[k] = lg_load(z + (j < to ? j : 0), to - j); }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) top = lg_top(v[k], top);
+    if (top > m) { s *= (double)lg_exp(m - top); m = top; }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) s += lg_sum(v[k], lg_base(m));
+  }
+  float M = lg_lanes_max<64>(m);
+  if ((tid & 63) == 0) red_m[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+  if (m != -INFINITY) s *= (double)lg_exp(m - lg_base(M));
+  s = lg_lanes_sum<64>(s);
+  if ((tid & 63) == 0) red_s[tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) {
+    part_m[row * parts + blockIdx.x] = M;
+    part_s[row * parts + blockIdx.x] = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
+  }
+}
+// ... and their join, a wave per row: what long_kernel does after its last barrier
+template <typename T, int MODE>
+__global__ void __launch_bounds__(64)
+join_kernel(Rows R, Policy P, Outs O, int parts, const float *__restrict__ part_m, const double *__restrict__ part_s) {
+  double add[3] = {0.0, 0.0, 0.0};
+  const int lane = (int)threadIdx.x;
+  const long long row = blockIdx.x;
+  const Row w = lg_row(R, row);
+  if (!w.counts || w.bad) lg_void(R, P, O, w, lane == 0, MODE == LG_POLICY, add);
+  else {
+    const float zy = (float)((const T *)R.z + row * R.ld)[w.y];
+    const float m = lane < parts ? part_m[row * parts + lane] : -INFINITY;
+    const float M = lg_lanes_max<64>(m);
+    double s = lane < parts ? part_s[row * parts + lane] : 0.0;
+    if (m != -INFINITY) s *= (double)lg_exp(m - lg_base(M));
+    s = lg_lanes_sum<64>(s);
+    lg_finish<T>(R, P, O, w, zy, M, s, lane == 0, MODE == LG_POLICY, add);
+  }
+  if (MODE == LG_POLICY) lg_partial<64>(P, add, (int)blockIdx.x);
 }
 
 // rows that count, of sequence blockIdx.y (of all rows without offsets), in gridDim.x parts
@@ -283,7 +515,7 @@ count_kernel(long long rows, const int *__restrict__ offset, const long long *__
 }
 
 __device__ __forceinline__ double lg_block_sum(double x, double *red) {
-  x = lg_wave_sum(x);
+  x = lg_lanes_sum<64>(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
@@ -339,8 +571,6 @@ pairs_kernel(int pairs, const double *__restrict__ sums, const float *__restrict
   if (threadIdx.x == 0) *loss = (float)(t / pairs);
 }
 
-constexpr int LG_GRID = 2048;
-
 int check_rows(const rs_logits *l, const char *name) {
   RS_REQUIRE(l && l->rows >= 0 && l->classes > 0 && l->classes <= 1 << 30 && l->ld >= l->classes && l->type >= 0 && l->type <= 2, "%s: bad size or type", name);
   RS_REQUIRE(l->sequences >= 0 && (!l->offset) == (l->sequences == 0), "%s: offsets and their number do not match", name);
@@ -352,19 +582,53 @@ Rows rows_of(const rs_logits *l) {
   return Rows{l->logits, l->rows, l->ld, l->classes, l->sequences, l->target, l->ignore_index, l->offset, l->bad_labels};
 }
 
-// waves of a row's team: one up to 1024 classes, a workgroup of 4 or 16 above
-int waves_of(int classes) { return classes <= 1024 ? 1 : (classes <= 16384 ? 4 : 16); }
-int grid_of(long long rows, int waves) {
-  const long long need = waves == 1 ? (rows + 3) / 4 : rows;
-  return (int)(need < LG_GRID ? need : LG_GRID);
+constexpr int LG_GRID = 2048;             // 8 workgroups of 256 threads on each of 256 CUs
+constexpr int LG_SHORT = 2048;            // classes of the longest row that a wave holds
+constexpr int LG_FEW = 256, LG_PARTS = 64;
+static_assert(LG_PARTS == RS_LOGITS_PARTS && LG_FEW == RS_LOGITS_FEW_ROWS, "room of the callers' scratch");
+
+int lesser(long long a, long long b) { return (int)(a < b ? a : b); }
+
+// Few long rows are cut so that about 512 workgroups share them, in pieces of 2048 logits at least; 1: not cut
+int parts_of(const rs_logits *l) {
+  if (l->rows > LG_FEW || l->classes <= 8192) return 1;
+  const int room = l->classes / 2048 < LG_PARTS ? l->classes / 2048 : LG_PARTS, want = (int)((512 + l->rows - 1) / l->rows);
+  return want < room ? want : room;
 }
 
-#define LG_WAVES(W, ...)                                    \
-  do {                                                      \
-    if (W == 1) { constexpr int WAVES = 1; __VA_ARGS__; }   \
-    else if (W == 4) { constexpr int WAVES = 4; __VA_ARGS__; } \
-    else { constexpr int WAVES = 16; __VA_ARGS__; }         \
-  } while (0)
+template <typename T, int MODE>
+int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &O, hipStream_t st) {
+  const int V = R.classes;
+#define LG_RUN_SHORT(L, N) { const int g = lesser((R.rows + 256 / L - 1) / (256 / L), LG_GRID); hipLaunchKernelGGL((short_kernel<T, MODE, L, N>), dim3(g), dim3(256), 0, st, R, P, O); return g; }
+  if (V <= 16) LG_RUN_SHORT(2, 1)
+  if (V <= 32) LG_RUN_SHORT(4, 1)
+  if (V <= 64) LG_RUN_SHORT(8, 1)
+  if (V <= 128) LG_RUN_SHORT(16, 1)
+  if (V <= 256) LG_RUN_SHORT(32, 1)
+  if (V <= 512) LG_RUN_SHORT(64, 1)
+  if (V <= 1024) LG_RUN_SHORT(64, 2)
+  if (V <= LG_SHORT) LG_RUN_SHORT(64, 4)
+#undef LG_RUN_SHORT
+  if constexpr (MODE == LG_BACK) {
+    constexpr int NV = 4;
+    const int parts = (V + 256 * LG_VEC * NV - 1) / (256 * LG_VEC * NV), g = lesser(R.rows * parts, 2 * LG_GRID);
+    hipLaunchKernelGGL((long_back_kernel<T, NV>), dim3(g), dim3(256), 0, st, R, O, parts);
+    return g;
+  } else {
+#define LG_RUN_LONG(TH, N, H) { const int g = lesser(R.rows, LG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
+    if constexpr (MODE == LG_POLICY) {       // (without a gradient too: the loss has the same bits either way)
+      if (V <= 4096) LG_RUN_LONG(256, 2, true)
+      if (V <= 8192) LG_RUN_LONG(256, 4, true)
+      if (V <= 16384) LG_RUN_LONG(512, 4, true)
+      if (V <= 32768) LG_RUN_LONG(1024, 4, true)
+      if (V <= 65536) LG_RUN_LONG(1024, 8, true)
+      if constexpr (sizeof(T) == 2) { if (V <= 131072) LG_RUN_LONG(1024, 16, true) }
+    }
+    LG_RUN_LONG(256, 4, false)
+#undef LG_RUN_LONG
+  }
+}
+
 #define LG_TYPE(K, ...)                                     \
   do {                                                      \
     if (K == 0) { typedef float T; __VA_ARGS__; }           \
@@ -372,16 +636,41 @@ int grid_of(long long rows, int waves) {
     else { typedef _Float16 T; __VA_ARGS__; }               \
   } while (0)
 
+// rows of any kind, cut or not; returns the number of workgroups that left partial sums
+template <int MODE>
+int run_rows(const rs_logits *l, const Policy &P, const Outs &O, void *scratch, hipStream_t st) {
+  const Rows R = rows_of(l);
+  const int parts = scratch ? parts_of(l) : 1;
+  int n = 0;
+  if (parts > 1) {
+    const int piece = ((l->classes + parts - 1) / parts + LG_VEC - 1) / LG_VEC * LG_VEC;
+    const int cut = (l->classes + piece - 1) / piece;
+    double *part_s = (double *)scratch;
+    float *part_m = (float *)(part_s + l->rows * cut);
+    LG_TYPE(l->type, hipLaunchKernelGGL((part_kernel<T, 2>), dim3(cut, (int)l->rows), dim3(256), 0, st, R, cut, piece, part_m, part_s);
+            hipLaunchKernelGGL((join_kernel<T, MODE>), dim3((int)l->rows), dim3(64), 0, st, R, P, O, cut, part_m, part_s));
+    n = (int)l->rows;
+    if (MODE == LG_POLICY && O.dz) {
+      Outs B = O;
+      B.coef = P.coef; B.up = nullptr; B.skip_unit = 0;
+      Rows Q = R;
+      Q.offset = nullptr; Q.sequences = 0;                     // (coef is per row, 0 for those behind the last sequence)
+      LG_TYPE(l->type, (launch_rows<T, LG_BACK>(l, Q, P, B, st)));
+    }
+  } else {
+    LG_TYPE(l->type, n = (launch_rows<T, MODE>(l, R, P, O, st)));
+  }
+  return n;
+}
+
 }  // namespace
 
-extern "C" int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64, float *stat, void *stream) {
+extern "C" int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64, float *stat, void *scratch, void *stream) {
   const int rc = check_rows(l, "rs_token_logprobs");
   if (rc != RS_OK) return rc;
   if (l->rows == 0) return RS_OK;
   RS_REQUIRE(logp || logp64, "rs_token_logprobs: null pointer");
-  const int w = waves_of(l->classes);
-  LG_TYPE(l->type, LG_WAVES(w, hipLaunchKernelGGL((rows_kernel<T, LG_LOGP, WAVES>), dim3(grid_of(l->rows, w)), dim3(WAVES < 4 ? 256 : WAVES * 64), 0,
-                                                  (hipStream_t)stream, rows_of(l), Policy{}, logp, logp64, (float2 *)stat, (T *)nullptr)));
+  run_rows<LG_LOGP>(l, Policy{}, Outs{logp, logp64, (float2 *)stat, nullptr, nullptr, nullptr, 0}, scratch, (hipStream_t)stream);
   RS_CHECK_LAUNCH("rs_token_logprobs");
   return RS_OK;
 }
@@ -392,9 +681,8 @@ extern "C" int rs_token_logprobs_backward(const rs_logits *l, const float *stat,
   if (rc != RS_OK) return rc;
   if (l->rows == 0) return RS_OK;
   RS_REQUIRE(stat && coef && dlogits, "rs_token_logprobs_backward: null pointer");
-  const int w = waves_of(l->classes);
-  LG_TYPE(l->type, LG_WAVES(w, hipLaunchKernelGGL((rows_backward_kernel<T, WAVES>), dim3(grid_of(l->rows, w)), dim3(WAVES < 4 ? 256 : WAVES * 64), 0,
-                                                  (hipStream_t)stream, rows_of(l), (const float2 *)stat, coef, gout, skip_unit, (T *)dlogits)));
+  const Outs O{nullptr, nullptr, (float2 *)stat, dlogits, coef, gout, skip_unit};
+  LG_TYPE(l->type, (launch_rows<T, LG_BACK>(l, rows_of(l), Policy{}, O, (hipStream_t)stream)));
   RS_CHECK_LAUNCH("rs_token_logprobs_backward");
   return RS_OK;
 }
@@ -430,16 +718,16 @@ extern "C" int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stre
   splits = splits < 1 ? 1 : (splits > 64 ? 64 : splits);
   RS_REQUIRE((long long)parts * splits <= p->counts_room, "rs_policy_loss: room for %d counts, %lld are needed", p->counts_room, parts * splits);
   RS_REQUIRE(parts <= 65535, "rs_policy_loss: %d sequences (at most 65535)", parts);
-  const int w = waves_of(l->classes), n = grid_of(l->rows, w);
-  RS_REQUIRE(3 * n <= p->partial_room, "rs_policy_loss: room for %d partial sums, %d are needed", p->partial_room, 3 * n);
+  RS_REQUIRE(p->partial_room >= RS_POLICY_PARTIAL, "rs_policy_loss: room for %d partial sums, %d are needed", p->partial_room, RS_POLICY_PARTIAL);
+  static_assert(RS_POLICY_PARTIAL >= 3 * LG_GRID, "room of the callers' partial sums");
   // (all rows of a token mean: those of the offsets' last sequence end them)
   hipLaunchKernelGGL(count_kernel, dim3((int)splits, parts), dim3(256), 0, st, l->rows,
                      l->offset ? (p->token_mean ? l->offset + l->sequences - 1 : l->offset) : nullptr, l->target, l->ignore_index, p->counts);
+  int n = 0;
   if (l->rows > 0) {
-    Policy P{p->old_logp, p->advantages, p->ref_logp, p->advantages_per_sequence, p->token_mean, p->low, p->high, p->kl_coef, p->counts, (int)splits,
-             p->coef, p->partial};
-    LG_TYPE(l->type, LG_WAVES(w, hipLaunchKernelGGL((rows_kernel<T, LG_POLICY, WAVES>), dim3(n), dim3(WAVES < 4 ? 256 : WAVES * 64), 0, st, rows_of(l), P,
-                                                    p->logp, (double *)nullptr, (float2 *)p->stat, (T *)p->dlogits)));
+    const Policy P{p->old_logp, p->advantages, p->ref_logp, p->advantages_per_sequence, p->token_mean, p->low, p->high, p->kl_coef, p->counts, (int)splits,
+                   p->coef, p->partial};
+    n = run_rows<LG_POLICY>(l, P, Outs{p->logp, nullptr, (float2 *)p->stat, p->dlogits, nullptr, nullptr, 0}, p->scratch, st);
   }
   hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(256), 0, st, n, p->partial, p->loss, p->stats);
   RS_CHECK_LAUNCH("rs_policy_loss");

@@ -25,6 +25,7 @@ from . import _lib, head
 P, c_int, c_ll, c_double = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POLICY_COUNTS, POLICY_PARTIAL = 64, 6144          # RS_POLICY_COUNTS, RS_POLICY_PARTIAL
+FEW_ROWS, PARTS = 256, 64                         # RS_LOGITS_FEW_ROWS, RS_LOGITS_PARTS
 
 PolicyLoss = namedtuple("PolicyLoss", "loss logp kl clip_fraction")
 PreferenceLoss = namedtuple("PreferenceLoss", "loss chosen_rewards rejected_rewards")
@@ -38,7 +39,7 @@ class LogitsDesc(ctypes.Structure):          # rs_logits
 class PolicyDesc(ctypes.Structure):          # rs_policy
     _fields_ = [("old_logp", P), ("advantages", P), ("ref_logp", P), ("advantages_per_sequence", c_int), ("token_mean", c_int), ("low", c_double),
                 ("high", c_double), ("kl_coef", c_double), ("counts", P), ("counts_room", c_int), ("partial", P), ("partial_room", c_int),
-                ("loss", P), ("stats", P), ("logp", P), ("dlogits", P), ("coef", P), ("stat", P)]
+                ("loss", P), ("stats", P), ("logp", P), ("dlogits", P), ("coef", P), ("stat", P), ("scratch", P)]
 
 
 def _logits(logits, target, offset):
@@ -93,15 +94,21 @@ def _new(logits, *shape, dtype=torch.float32):
     return torch.empty(shape, dtype=dtype, device=logits.device)
 
 
+def _scratch(logits):
+    """room for the pieces of a few long rows, or None"""
+    rows, classes = logits.shape
+    return None if rows > FEW_ROWS or classes <= 8192 else _new(logits, 3 * PARTS * rows)
+
+
 class _TokenLogprobs(Function):
     @staticmethod
     def forward(ctx, logits, target, ignore_index, grad):
         rows = logits.shape[0]
         logp = _new(logits, rows)
-        stat = _new(logits, rows, 2) if grad else None
+        stat, scratch = _new(logits, rows, 2) if grad else None, _scratch(logits)
         with torch.cuda.device(logits.device):
             _lib.call("rs_token_logprobs", ctypes.byref(_desc(logits, target, ignore_index, None)), logp.data_ptr(), None,
-                      None if stat is None else stat.data_ptr(), _lib.current_stream())
+                      None if stat is None else stat.data_ptr(), None if scratch is None else scratch.data_ptr(), _lib.current_stream())
         if stat is not None:
             ctx.save_for_backward(logits, target, stat)
             ctx.ignore_index = ignore_index
@@ -129,7 +136,9 @@ def _sequences(logits, target, offset, ignore_index, average, stat):
     logp, sums = _new(logits, logits.shape[0], dtype=torch.float64), _new(logits, n, dtype=torch.float64)
     out, each = _new(logits, n), _new(logits, n)
     desc = _desc(logits, target, ignore_index, offset)
-    _lib.call("rs_token_logprobs", ctypes.byref(desc), None, logp.data_ptr(), None if stat is None else stat.data_ptr(), _lib.current_stream())
+    scratch = _scratch(logits)
+    _lib.call("rs_token_logprobs", ctypes.byref(desc), None, logp.data_ptr(), None if stat is None else stat.data_ptr(),
+              None if scratch is None else scratch.data_ptr(), _lib.current_stream())
     _lib.call("rs_sequence_sums", ctypes.byref(desc), logp.data_ptr(), int(average), sums.data_ptr(), out.data_ptr(), each.data_ptr(),
               _lib.current_stream())
     return desc, sums, out, each
@@ -220,6 +229,9 @@ class _Policy(Function):
                        advantages_per_sequence=int(adv.dim() == 2), token_mean=int(token_mean), low=low, high=high, kl_coef=kl_coef,
                        counts=counts.data_ptr(), counts_room=room, partial=partial.data_ptr(), partial_room=POLICY_PARTIAL, loss=loss.data_ptr(),
                        stats=stats.data_ptr(), logp=logp.data_ptr())
+        scratch = _scratch(logits)
+        if scratch is not None:
+            p.scratch = scratch.data_ptr()
         if grad and rows:
             p.dlogits, p.coef, p.stat = d.data_ptr(), row.data_ptr(), row.data_ptr() + 4 * rows
         with torch.cuda.device(logits.device):

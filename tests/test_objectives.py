@@ -40,11 +40,11 @@ def test_entry_points_report_bad_arguments():
     for bad in (dict(rows=-1), dict(classes=0), dict(ld=7), dict(type=3), dict(offset=256), dict(sequences=2), dict(logits=None), dict(target=None),
                 dict(classes=(1 << 30) + 1, ld=1 << 31), dict(rows=1 << 31, offset=256, sequences=1)):
         with pytest.raises(_lib.RepSurfHipError, match="rs_token_logprobs"):
-            _lib.call("rs_token_logprobs", rows(**bad), 256, None, None, None)
+            _lib.call("rs_token_logprobs", rows(**bad), 256, None, None, None, None)
         with pytest.raises(_lib.RepSurfHipError):
             _lib.call("rs_token_logprobs_backward", rows(**bad), 256, 256, None, 0, 256, None)
     with pytest.raises(_lib.RepSurfHipError, match="null"):
-        _lib.call("rs_token_logprobs", rows(), None, None, None, None)
+        _lib.call("rs_token_logprobs", rows(), None, None, None, None, None)
     with pytest.raises(_lib.RepSurfHipError, match="null"):
         _lib.call("rs_token_logprobs_backward", rows(), None, 256, None, 0, 256, None)
     with pytest.raises(_lib.RepSurfHipError, match="null"):
@@ -59,17 +59,17 @@ def test_entry_points_report_bad_arguments():
         return ctypes.byref(O.PolicyDesc(**d))
 
     for bad in (dict(loss=None), dict(stats=None), dict(partial=None), dict(counts=None), dict(old_logp=None), dict(advantages=None), dict(dlogits=256),
-                dict(coef=256), dict(token_mean=0), dict(advantages_per_sequence=1), dict(counts_room=0)):
+                dict(coef=256), dict(token_mean=0), dict(advantages_per_sequence=1), dict(counts_room=0), dict(partial_room=6143)):
         with pytest.raises(_lib.RepSurfHipError, match="rs_policy_loss"):
             _lib.call("rs_policy_loss", rows(), policy(**bad), None)
-    _lib.call("rs_token_logprobs", rows(rows=0), 256, None, None, None)          # nothing to do
+    _lib.call("rs_token_logprobs", rows(rows=0), 256, None, None, None, None)          # nothing to do
     _lib.call("rs_token_logprobs_backward", rows(rows=0), 256, 256, None, 0, 256, None)
 
 
 def test_structs_match_the_header(tmp_path):
     pairs = {"rs_logits": O.LogitsDesc, "rs_policy": O.PolicyDesc}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "repsurf_hip.h"', 'int main(void) {',
-             f'if (RS_POLICY_COUNTS != {O.POLICY_COUNTS} || RS_POLICY_PARTIAL != {O.POLICY_PARTIAL}) return 1;']
+             f'if (RS_POLICY_COUNTS != {O.POLICY_COUNTS} || RS_POLICY_PARTIAL != {O.POLICY_PARTIAL} || RS_LOGITS_FEW_ROWS != {O.FEW_ROWS} || RS_LOGITS_PARTS != {O.PARTS}) return 1;']
     for c, cls in pairs.items():
         lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
         lines += [f'printf("{c} {f} %zu\\n", offsetof({c}, {f}));' for f, _ in cls._fields_]
