@@ -48,41 +48,67 @@ def _logits(logits, target, offset):
         raise ValueError(f"objectives: logits must be (rows, classes), got {tuple(logits.shape)}")
     if logits.dtype not in _TYPES:
         raise TypeError(f"objectives: logits must be fp32, bf16 or fp16, got {logits.dtype}")
-    if target.shape != logits.shape[:1] or target.is_floating_point():
+    if target.dim() != 1 or target.shape[0] != logits.shape[0] or target.is_floating_point():
         raise ValueError(f"objectives: target must hold one class index per row, got {tuple(target.shape)} {target.dtype}")
     if offset is not None and (offset.dim() != 1 or offset.numel() < 1 or offset.is_floating_point()):
         raise ValueError("objectives: offset must be the (B,) running row ends")
-    for t in (logits, target, offset):
-        if t is not None and t.device != logits.device:
-            raise ValueError("objectives: all tensors must be on the logits' device")
-    if not logits.is_cuda:
+    device = logits.device
+    if target.device != device or (offset is not None and offset.device != device):
+        raise ValueError("objectives: all tensors must be on the logits' device")
+    if device.type != "cuda":
         raise _lib.RepSurfHipError("repsurf_amd.objectives run on the HIP device only (got a CPU tensor); there is no CPU fallback")
-    if logits.shape[0] and (logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]):
+    if not logits.is_contiguous() and (logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]):
         logits = logits.contiguous()
-    target = target.to(torch.int64).contiguous()
-    if offset is not None:
-        offset = offset.to(torch.int32).contiguous()
-    return logits, target, offset
+    return logits, _as(target, torch.int64), None if offset is None else _as(offset, torch.int32)
+
+
+def _as(t, dtype):
+    """data (not differentiated) as a dense tensor of a type"""
+    if t.dtype is dtype and t.is_contiguous():
+        return t
+    return t.detach().to(dtype).contiguous()
 
 
 def _values(name, t, shape, logits):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"objectives: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != logits.device:
         raise ValueError("objectives: all tensors must be on the logits' device")
-    return t.detach().to(torch.float32).contiguous()
+    return _as(t, torch.float32)
+
+
+_bad = {}
 
 
 def _desc(logits, target, ignore_index, offset):
     rows, classes = logits.shape
-    return LogitsDesc(logits=logits.data_ptr(), rows=rows, ld=max(logits.stride(0), classes), classes=classes, type=_TYPES[logits.dtype],
-                      target=target.data_ptr(), ignore_index=int(ignore_index), offset=None if offset is None else offset.data_ptr(),
-                      sequences=0 if offset is None else offset.numel(), bad_labels=head._bad_counter(logits.device).data_ptr())
+    device = logits.device
+    bad = _bad.get(device.index)
+    if bad is None:
+        bad = _bad[device.index] = head._bad_counter(device).data_ptr()        # (lives as long as the process)
+    return LogitsDesc(logits.data_ptr(), rows, max(logits.stride(0), classes), classes, _TYPES[logits.dtype], target.data_ptr(), ignore_index,
+                      None if offset is None else offset.data_ptr(), 0 if offset is None else offset.numel(), bad)
 
 
-def _backward(desc, logits, stat, coef, gout, skip_unit, out):
-    _lib.call("rs_token_logprobs_backward", ctypes.byref(desc), stat.data_ptr(), coef.data_ptr(), None if gout is None else gout.data_ptr(),
-              skip_unit, out.data_ptr(), _lib.current_stream())
+def _call(device, name, *args):
+    """an ABI call on the current stream of the tensors' device"""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.current_stream())
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.current_stream())
+
+
+def _backward(ctx, logits, target, offset, work, coef, gout, skip_unit=0, out=None):
+    """from the tensors as autograd hands them back (a hook may have moved them); the rows' stat lies in `work`, ctx.stat floats from its
+    start; coef: an address"""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    desc = ctx.desc
+    desc.logits, desc.ld, desc.target = logits.data_ptr(), max(logits.stride(0), logits.shape[1]), target.data_ptr()
+    desc.offset, desc.sequences = (None, 0) if offset is None else (offset.data_ptr(), offset.numel())
+    _call(logits.device, "rs_token_logprobs_backward", ctypes.byref(desc), work.data_ptr() + 4 * ctx.stat, coef,
+          None if gout is None else _as(gout, torch.float32).data_ptr(), skip_unit, out.data_ptr())
     return out
 
 
@@ -94,33 +120,33 @@ def _new(logits, *shape, dtype=torch.float32):
     return torch.empty(shape, dtype=dtype, device=logits.device)
 
 
-def _scratch(logits):
-    """room for the pieces of a few long rows, or None"""
+def _scratch_floats(logits):
+    """room (a multiple of 8 bytes) for the pieces of a few long rows"""
     rows, classes = logits.shape
-    return None if rows > FEW_ROWS or classes <= 8192 else _new(logits, 3 * PARTS * rows)
+    return 0 if rows > FEW_ROWS or classes <= 8192 else 3 * PARTS * rows
 
 
 class _TokenLogprobs(Function):
     @staticmethod
     def forward(ctx, logits, target, ignore_index, grad):
         rows = logits.shape[0]
+        room = _scratch_floats(logits)
         logp = _new(logits, rows)
-        stat, scratch = _new(logits, rows, 2) if grad else None, _scratch(logits)
-        with torch.cuda.device(logits.device):
-            _lib.call("rs_token_logprobs", ctypes.byref(_desc(logits, target, ignore_index, None)), logp.data_ptr(), None,
-                      None if stat is None else stat.data_ptr(), None if scratch is None else scratch.data_ptr(), _lib.current_stream())
-        if stat is not None:
-            ctx.save_for_backward(logits, target, stat)
-            ctx.ignore_index = ignore_index
+        work = _new(logits, room + (2 * rows if grad else 0)) if room or grad else None          # scratch, then stat
+        desc = _desc(logits, target, ignore_index, None)
+        _call(logits.device, "rs_token_logprobs", ctypes.byref(desc), logp.data_ptr(), None, work.data_ptr() + 4 * room if grad else None,
+              work.data_ptr() if room else None)
+        if grad:
+            ctx.save_for_backward(logits, target, work)
+            ctx.desc, ctx.stat = desc, room
         return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, target, stat = ctx.saved_tensors
-        with torch.cuda.device(logits.device):
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            return _backward(_desc(logits, target, ctx.ignore_index, None), logits, stat, g.to(torch.float32).contiguous(), None, 0, d), None, None, None
+        logits, target, work = ctx.saved_tensors
+        g = _as(g, torch.float32)
+        return _backward(ctx, logits, target, None, work, g.data_ptr(), None), None, None, None
 
 
 def token_logprobs(logits, target, ignore_index=-100):
@@ -130,39 +156,38 @@ def token_logprobs(logits, target, ignore_index=-100):
     return _TokenLogprobs.apply(logits, target, ignore_index, _wanted(logits))
 
 
-def _sequences(logits, target, offset, ignore_index, average, stat):
-    """-> (desc, sums fp64, sums fp32, each): a row's factor in its sequence's sum"""
-    n = offset.numel()
-    logp, sums = _new(logits, logits.shape[0], dtype=torch.float64), _new(logits, n, dtype=torch.float64)
-    out, each = _new(logits, n), _new(logits, n)
+def _sequences(logits, target, offset, ignore_index, average, extra=0):
+    """-> (desc, out fp32, buffer, places): what the sequences of a packed batch add up to.  One buffer holds the rows' fp64
+    log-probabilities, the sequences' fp64 sums, scratch, the rows' stat, and the sequences' factors, at these places (in floats)."""
+    rows, n, room = logits.shape[0], offset.numel(), _scratch_floats(logits)
+    sizes = dict(logp=2 * rows, sums=2 * n, scratch=room, stat=2 * rows, each=n, extra=extra)
+    buf, out = _new(logits, sum(sizes.values())), _new(logits, n)
+    places, at, start = {}, 0, buf.data_ptr()
+    for k, v in sizes.items():
+        places[k] = at
+        at += v
+    of = {k: start + 4 * v for k, v in places.items()}
     desc = _desc(logits, target, ignore_index, offset)
-    scratch = _scratch(logits)
-    _lib.call("rs_token_logprobs", ctypes.byref(desc), None, logp.data_ptr(), None if stat is None else stat.data_ptr(),
-              None if scratch is None else scratch.data_ptr(), _lib.current_stream())
-    _lib.call("rs_sequence_sums", ctypes.byref(desc), logp.data_ptr(), int(average), sums.data_ptr(), out.data_ptr(), each.data_ptr(),
-              _lib.current_stream())
-    return desc, sums, out, each
+    _call(logits.device, "rs_token_logprobs", ctypes.byref(desc), None, of["logp"], of["stat"], of["scratch"] if room else None)
+    _call(logits.device, "rs_sequence_sums", ctypes.byref(desc), of["logp"], int(average), of["sums"], out.data_ptr(), of["each"])
+    return desc, out, buf, places
 
 
 class _SequenceLogprobs(Function):
     @staticmethod
     def forward(ctx, logits, target, offset, ignore_index, average, grad):
-        stat = _new(logits, logits.shape[0], 2) if grad else None
-        with torch.cuda.device(logits.device):
-            _, _, out, each = _sequences(logits, target, offset, ignore_index, average, stat)
-        if stat is not None:
-            ctx.save_for_backward(logits, target, offset, stat, each)
-            ctx.ignore_index = ignore_index
+        desc, out, buf, places = _sequences(logits, target, offset, ignore_index, average)
+        if grad:
+            ctx.save_for_backward(logits, target, offset, buf)
+            ctx.desc, ctx.stat = desc, places["stat"]
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, target, offset, stat, each = ctx.saved_tensors
-        with torch.cuda.device(logits.device):
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            d = _backward(_desc(logits, target, ctx.ignore_index, offset), logits, stat, g.to(torch.float32) * each, None, 0, d)
-        return d, None, None, None, None, None
+        logits, target, offset, buf = ctx.saved_tensors
+        coef = _as(g, torch.float32) * buf[buf.numel() - offset.numel():]
+        return (_backward(ctx, logits, target, offset, buf, coef.data_ptr(), None),) + (None,) * 5
 
 
 def sequence_logprobs(logits, target, offset, ignore_index=-100, average=False):
@@ -176,26 +201,21 @@ class _Preference(Function):
     @staticmethod
     def forward(ctx, logits, target, offset, ref, beta, smoothing, average, ignore_index, grad):
         n = offset.numel()
-        stat = _new(logits, logits.shape[0], 2) if grad else None
-        loss, rewards, coef = _new(logits), _new(logits, n), _new(logits, n)
-        with torch.cuda.device(logits.device):
-            _, sums, _, each = _sequences(logits, target, offset, ignore_index, average, stat)
-            _lib.call("rs_preference_pairs", n // 2, sums.data_ptr(), each.data_ptr(), ref.data_ptr(), float(beta), float(smoothing), loss.data_ptr(),
-                      rewards.data_ptr(), coef.data_ptr(), _lib.current_stream())
-        if stat is not None:
-            ctx.save_for_backward(logits, target, offset, stat, coef)
-            ctx.ignore_index = ignore_index
+        desc, rewards, buf, places = _sequences(logits, target, offset, ignore_index, average, extra=n)
+        loss, start = _new(logits), buf.data_ptr()
+        _call(logits.device, "rs_preference_pairs", n // 2, start + 4 * places["sums"], start + 4 * places["each"], ref.data_ptr(), beta, smoothing,
+              loss.data_ptr(), rewards.data_ptr(), start + 4 * places["extra"])
+        if grad:
+            ctx.save_for_backward(logits, target, offset, buf)
+            ctx.desc, ctx.stat, ctx.coef = desc, places["stat"], places["extra"]
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _):
-        logits, target, offset, stat, coef = ctx.saved_tensors
-        with torch.cuda.device(logits.device):
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            d = _backward(_desc(logits, target, ctx.ignore_index, offset), logits, stat, coef, g.to(torch.float32).contiguous(), 0, d)
-        return (d,) + (None,) * 8
+        logits, target, offset, buf = ctx.saved_tensors
+        return (_backward(ctx, logits, target, offset, buf, buf.data_ptr() + 4 * ctx.coef, g),) + (None,) * 8
 
 
 def preference_loss(logits, target, offset, ref_logps, beta=0.1, label_smoothing=0.0, average=False, ignore_index=-100):
@@ -211,7 +231,7 @@ def preference_loss(logits, target, offset, ref_logps, beta=0.1, label_smoothing
     if not 0.0 <= label_smoothing <= 0.5:
         raise ValueError("preference_loss: label_smoothing must lie in [0, 0.5]")
     ref = _values("ref_logps", ref_logps, (n,), logits)
-    loss, rewards = _Preference.apply(logits, target, offset, ref, beta, label_smoothing, average, ignore_index, _wanted(logits))
+    loss, rewards = _Preference.apply(logits, target, offset, ref, float(beta), float(label_smoothing), average, ignore_index, _wanted(logits))
     return PreferenceLoss(loss, rewards[: n // 2], rewards[n // 2:])
 
 
@@ -220,45 +240,39 @@ class _Policy(Function):
     def forward(ctx, logits, target, old, adv, ref, offset, low, high, kl_coef, token_mean, ignore_index, grad):
         rows = logits.shape[0]
         loss, stats, logp = _new(logits), _new(logits, 2), _new(logits, rows)
+        room, counts = _scratch_floats(logits), POLICY_COUNTS * (1 if token_mean else offset.numel())
+        # one buffer: partial sums (fp64), scratch, counts, then the rows' stat (pairs: at an even place) and coef
+        work = _new(logits, 2 * POLICY_PARTIAL + room + counts + (3 * rows if grad else 0))
+        at = work.data_ptr()
+        scratch = at + 8 * POLICY_PARTIAL
+        count_at = scratch + 4 * room
+        stat = count_at + 4 * counts
+        coef = stat + 8 * rows
         d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
-        row = _new(logits, rows, 3) if grad else None                # coef, and stat behind it
-        room = POLICY_COUNTS * (1 if token_mean else offset.numel())
-        counts, partial = _new(logits, room, dtype=torch.int32), _new(logits, POLICY_PARTIAL, dtype=torch.float64)
+        held = grad and rows > 0
         desc = _desc(logits, target, ignore_index, offset)
-        p = PolicyDesc(old_logp=old.data_ptr(), advantages=adv.data_ptr(), ref_logp=None if ref is None else ref.data_ptr(),
-                       advantages_per_sequence=int(adv.dim() == 2), token_mean=int(token_mean), low=low, high=high, kl_coef=kl_coef,
-                       counts=counts.data_ptr(), counts_room=room, partial=partial.data_ptr(), partial_room=POLICY_PARTIAL, loss=loss.data_ptr(),
-                       stats=stats.data_ptr(), logp=logp.data_ptr())
-        scratch = _scratch(logits)
-        if scratch is not None:
-            p.scratch = scratch.data_ptr()
-        if grad and rows:
-            p.dlogits, p.coef, p.stat = d.data_ptr(), row.data_ptr(), row.data_ptr() + 4 * rows
-        with torch.cuda.device(logits.device):
-            _lib.call("rs_policy_loss", ctypes.byref(desc), ctypes.byref(p), _lib.current_stream())
+        p = PolicyDesc(old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr(), int(adv.dim() == 2), int(token_mean), low, high, kl_coef,
+                       count_at, counts, at, POLICY_PARTIAL, loss.data_ptr(), stats.data_ptr(), logp.data_ptr(), d.data_ptr() if held else None,
+                       coef if held else None, stat if held else None, scratch if room else None)
+        _call(logits.device, "rs_policy_loss", ctypes.byref(desc), ctypes.byref(p))
         if grad:
-            ctx.save_for_backward(logits, target, offset, row)
-            ctx.d, ctx.ignore_index = d, ignore_index
+            ctx.save_for_backward(logits, target, work)
+            ctx.d, ctx.desc, ctx.stat = d, desc, (stat - at) // 4
         ctx.mark_non_differentiable(logp, stats)
         return loss, logp, stats
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, *_):
-        logits, target, offset, row = ctx.saved_tensors
+        logits, target, work = ctx.saved_tensors
         d, first = ctx.d, ctx.d is not None
         ctx.d = None                       # handed out once: a second pass over a retained graph computes it again
-        one = head._unit.get(str(logits.device))
+        one = head._unit.get(str(logits.device)) if head._unit else None
         if first and ((one is not None and g.data_ptr() == one.data_ptr()) or logits.shape[0] == 0):      # loss.backward(unit_gradient(device))
             return (d,) + (None,) * 11
-        with torch.cuda.device(logits.device):
-            if not first:
-                d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            if logits.shape[0]:
-                # per-row coefficients: the offsets were taken into account when they were made
-                _lib.call("rs_token_logprobs_backward", ctypes.byref(_desc(logits, target, ctx.ignore_index, None)), row.data_ptr() + 4 * logits.shape[0],
-                          row.data_ptr(), g.to(torch.float32).contiguous().data_ptr(), int(first), d.data_ptr(), _lib.current_stream())
-        return (d,) + (None,) * 11
+        # coef is per row, 0 for the rows behind the last sequence: no offsets
+        coef = work.data_ptr() + 4 * (ctx.stat + 2 * logits.shape[0])
+        return (_backward(ctx, logits, target, None, work, coef, g, int(first), d),) + (None,) * 11
 
 
 def policy_loss(logits, target, old_logp, advantages, ref_logp=None, offset=None, clip=(0.2, 0.2), kl_coef=0.0, reduction="token", ignore_index=-100):
@@ -288,4 +302,4 @@ def policy_loss(logits, target, old_logp, advantages, ref_logp=None, offset=None
     ref = None if ref_logp is None else _values("ref_logp", ref_logp, (rows,), logits)
     loss, logp, stats = _Policy.apply(logits, target, old, adv, ref, offset, low, high, float(kl_coef), reduction == "token", ignore_index,
                                       _wanted(logits))
-    return PolicyLoss(loss, logp, stats[0], stats[1])
+    return PolicyLoss(loss, logp, *stats.unbind())

@@ -432,6 +432,21 @@ def test_captured_replays_are_the_eager_calls(classes, dtype):
     assert torch.isfinite(live[0])
 
 
+def test_saved_tensors_that_a_hook_moves():
+    """the backward passes read what autograd hands back, not where the forward pass found it"""
+    from repsurf_amd import objectives
+    z, y, _, old, adv, _ = policy_case([30, 20], 2, 1500, torch.bfloat16, 61)
+    y, old, adv, off = y.cuda(), old.cuda(), adv.cuda(), ends([30, 20])
+    calls = (lambda: objectives.token_logprobs(z, y).sum(), lambda: objectives.sequence_logprobs(z, y, off, average=True).sum(),
+             lambda: objectives.preference_loss(z, y, off, old[:2]).loss, lambda: objectives.policy_loss(z, y, old, adv, offset=off).loss * 0.5)
+    want = [torch.autograd.grad(f(), z)[0] for f in calls]
+    for f, w in zip(calls, want):
+        with torch.autograd.graph.save_on_cpu():
+            loss = f()
+        junk = [torch.full((52, 1500), 7.0, device="cuda") for _ in range(4)]
+        assert torch.equal(torch.autograd.grad(loss, z)[0], w) and len(junk) == 4
+
+
 def test_two_streams_at_once():
     from repsurf_amd import objectives
     cases = [policy_case([300, 200], 5, c, torch.bfloat16, 41 + c) for c in (600, 30001)]
