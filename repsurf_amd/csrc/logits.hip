@@ -33,33 +33,41 @@ struct Policy {
 };
 
 constexpr int LG_VEC = 8;
-template <typename T> struct Vec { T x[LG_VEC]; };
-// 8 consecutive logits, aligned to one of them: global loads and stores of this device need no more
+// 8 consecutive logits as the words they come in: two to a register in 16 bits
+template <typename T> struct Vec { unsigned w[LG_VEC * sizeof(T) / 4]; };
+__device__ __forceinline__ float lg_get(const Vec<float> &v, int i) { return __uint_as_float(v.w[i]); }
+__device__ __forceinline__ float lg_get(const Vec<__bf16> &v, int i) { return __uint_as_float(i & 1 ? v.w[i >> 1] & 0xFFFF0000u : v.w[i >> 1] << 16); }
+__device__ __forceinline__ float lg_get(const Vec<_Float16> &v, int i) {
+  return (float)__builtin_bit_cast(_Float16, (unsigned short)(i & 1 ? v.w[i >> 1] >> 16 : v.w[i >> 1]));
+}
+// aligned to one logit: global loads and stores of this device need no more
 template <typename T>
 __device__ __forceinline__ Vec<T> lg_load(const T *p, int left) {
   Vec<T> v;
   if (left >= LG_VEC) __builtin_memcpy(&v, p, sizeof(v));
   else {
+    T x[LG_VEC];
 #pragma unroll
-    for (int i = 0; i < LG_VEC; ++i) v.x[i] = i < left ? p[i] : (T)-INFINITY;
+    for (int i = 0; i < LG_VEC; ++i) x[i] = i < left ? p[i] : (T)-INFINITY;
+    __builtin_memcpy(&v, x, sizeof(v));
   }
   return v;
 }
 template <typename T>
 __device__ __forceinline__ void lg_store(T *p, int left, const float *x) {
-  Vec<T> v;
+  T v[LG_VEC];
 #pragma unroll
-  for (int i = 0; i < LG_VEC; ++i) v.x[i] = (T)x[i];
-  if (left >= LG_VEC) __builtin_memcpy(p, &v, sizeof(v));
+  for (int i = 0; i < LG_VEC; ++i) v[i] = (T)x[i];
+  if (left >= LG_VEC) __builtin_memcpy(p, v, sizeof(v));
   else {
 #pragma unroll
-    for (int i = 0; i < LG_VEC; ++i) if (i < left) p[i] = v.x[i];
+    for (int i = 0; i < LG_VEC; ++i) if (i < left) p[i] = v[i];
   }
 }
 template <typename T>
 __device__ __forceinline__ float lg_top(const Vec<T> &v, float m) {
 #pragma unroll
-  for (int i = 0; i < LG_VEC; ++i) m = fmaxf(m, (float)v.x[i]);
+  for (int i = 0; i < LG_VEC; ++i) m = fmaxf(m, lg_get(v, i));
   return m;
 }
 
@@ -72,7 +80,7 @@ template <typename T>
 __device__ __forceinline__ double lg_sum(const Vec<T> &v, float base) {
   float e[LG_VEC];
 #pragma unroll
-  for (int i = 0; i < LG_VEC; ++i) e[i] = lg_exp((float)v.x[i] - base);
+  for (int i = 0; i < LG_VEC; ++i) e[i] = lg_exp(lg_get(v, i) - base);
   return (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
 }
 // c ([j = y] - exp(z_j - base) inv), scale = -c inv; j: the index of v's first logit
@@ -80,8 +88,8 @@ template <typename T>
 __device__ __forceinline__ void lg_gradient(T *p, int left, const Vec<T> &v, float base, float scale, float c, int j, int y) {
   float g[LG_VEC];
 #pragma unroll
-  for (int i = 0; i < LG_VEC; ++i) g[i] = lg_exp((float)v.x[i] - base) * scale;
-  if (((j ^ y) & ~(LG_VEC - 1)) == 0) {
+  for (int i = 0; i < LG_VEC; ++i) g[i] = lg_exp(lg_get(v, i) - base) * scale;
+  if ((unsigned)(y - j) < (unsigned)LG_VEC) {
 #pragma unroll
     for (int i = 0; i < LG_VEC; ++i) g[i] += j + i == y ? c : 0.f;
   }
@@ -98,11 +106,8 @@ __device__ __forceinline__ void lg_fill(T *p, int left, float x) {
 // row in 16 bits, and a kernel that holds rows would spill.
 template <typename T>
 __device__ __forceinline__ void lg_forget(Vec<T> &v) {
-  unsigned w[sizeof(v) / 4];
-  __builtin_memcpy(w, &v, sizeof(v));
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(v) / 4); ++i) asm volatile("" : "+v"(w[i]));
-  __builtin_memcpy(&v, w, sizeof(v));
+  for (int i = 0; i < (int)(sizeof(v) / 4); ++i) asm volatile("" : "+v"(v.w[i]));
 }
 // the value that exponents are taken against: of a row that holds nothing but -infinity, 0 (exp(-inf - 0) = 0, and 0 / 0 follows)
 __device__ __forceinline__ float lg_base(float m) { return m == -INFINITY ? 0.f : m; }
@@ -221,22 +226,27 @@ __device__ __forceinline__ float lg_void(const Rows &R, const Policy &P, const O
   }
   return fill;
 }
-// what follows from a row's M and s.  All lanes of a team compute it: it costs a wave the same as one lane does.
-template <typename T>
-__device__ __forceinline__ float lg_finish(const Rows &R, const Policy &P, const Outs &O, const Row &w, float zy, float M, double s, bool first, int policy,
+// what the policy loss needs beside a row's logits: asked for before them
+struct Pre {
+  double w;
+  float old, adv, ref;
+};
+__device__ __forceinline__ Pre lg_pre(const Rows &R, const Policy &P, const Row &w) {
+  return Pre{lg_weight(R, P, w.owner), P.old_logp[w.at], P.adv[P.adv_per_sequence ? (long long)w.owner : w.at], P.ref ? P.ref[w.at] : 0.f};
+}
+// what follows from a row's M and s; `first`: the lane that writes it down
+__device__ __forceinline__ float lg_finish(const Policy &P, const Outs &O, long long row, const Pre &pre, float zy, float M, double s, bool first, int policy,
                                            double *add) {
   const double lp = (double)zy - (double)M - lg_log64(s);
   float c = 0.f;
   double mine[3] = {0.0, 0.0, 0.0};
-  if (policy)
-    c = (float)lg_policy(P, lg_weight(R, P, w.owner), lp, (double)P.old_logp[w.at], (double)P.adv[P.adv_per_sequence ? (long long)w.owner : w.at],
-                         P.ref ? (double)P.ref[w.at] : 0.0, mine);
+  if (policy) c = (float)lg_policy(P, pre.w, lp, (double)pre.old, (double)pre.adv, (double)pre.ref, mine);
   if (first) {
-    if (O.logp) O.logp[w.at] = (float)lp;
-    if (O.logp64) O.logp64[w.at] = lp;
-    if (O.stat) O.stat[w.at] = make_float2(M, 1.f / (float)s);
+    if (O.logp) O.logp[row] = (float)lp;
+    if (O.logp64) O.logp64[row] = lp;
+    if (O.stat) O.stat[row] = make_float2(M, 1.f / (float)s);
     if (policy) {
-      if (P.coef) P.coef[w.at] = c;
+      if (P.coef) P.coef[row] = c;
       add[0] += mine[0]; add[1] += mine[1]; add[2] += mine[2];
     }
   }
@@ -259,71 +269,118 @@ __device__ __forceinline__ void lg_partial(const Policy &P, const double *add, i
   }
 }
 
-// Rows of up to 2048 classes: LANES neighbouring lanes hold a row in NV vectors of 8 per lane; one read, one write.  With 13 classes a wave
-// works on 32 rows at once, so the fp64 steps of a row cost a 32nd of a wave's.
+// Rows of up to 4096 classes: LANES neighbouring lanes hold a row in NV vectors of 8 per lane; one read, one write.  A team takes SUB rows
+// before the fp64 steps, which its first SUB lanes then do for a row each: with 13 classes (2 lanes, 2 rows) every lane of a wave works
+// on a row of its own.
 template <typename T, int MODE, int LANES, int NV>
 __global__ void __launch_bounds__(256)
 short_kernel(Rows R, Policy P, Outs O) {
   constexpr int TEAMS = 256 / LANES;
+  constexpr int ROOM = MODE == LG_POLICY ? (8 / NV > 0 ? 8 / NV : 1) : 1, SUB = LANES < ROOM ? LANES : ROOM;
   const float up = MODE == LG_BACK && O.up ? *O.up : 1.f;
   if (MODE == LG_BACK && O.skip_unit && up == 1.f) return;
   const int team = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES, V = R.classes;
   double add[3] = {0.0, 0.0, 0.0};
-  for (long long first = (long long)blockIdx.x * TEAMS; first < R.rows; first += (long long)gridDim.x * TEAMS) {
-    const long long row = first + team;
-    const bool live = row < R.rows;                            // (all lanes take part in the exchanges below)
-    Row w{row, 0, 0, false, false};
-    if (live) w = lg_row(R, row);
-    const bool in = w.counts && !w.bad;
-    const T *__restrict__ z = (const T *)R.z + row * R.ld;
-    T *__restrict__ dz = O.dz ? (T *)O.dz + row * V : nullptr;
-    Vec<T> v[NV];
-    float c = 0.f, M = -INFINITY, inv = 0.f;
+  for (long long first = (long long)blockIdx.x * (TEAMS * SUB); first < R.rows; first += (long long)gridDim.x * (TEAMS * SUB)) {
+    Vec<T> v[SUB][NV];
+    Row w[SUB];
+    bool in[SUB];
+    float zy[SUB];
+    Row mine{0, 0, 0, false, false};                           // the row whose fp64 steps this lane does
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int j = (k * LANES + lane) * LG_VEC;
-      v[k] = lg_load(z + j, in ? V - j : 0);
-    }
-    if (MODE == LG_BACK) {
-      if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w.owner : row] * up;
-      if (in) { const float2 st = O.stat[row]; M = st.x; inv = st.y; }
-    } else {
-      const float zy = in ? (float)z[w.y] : 0.f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) { M = lg_top(v[k], M); if (NV > 1) lg_forget(v[k]); }
-      M = lg_lanes_max<LANES>(M);
-      double s = 0.0;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) { s += lg_sum(v[k], lg_base(M)); if (NV > 1) lg_forget(v[k]); }
-      s = lg_lanes_sum<LANES>(s);
-      if (in) c = lg_finish<T>(R, P, O, w, zy, M, s, lane == 0, MODE == LG_POLICY, add);
-      else if (live) c = lg_void(R, P, O, w, lane == 0, MODE == LG_POLICY, add);
-      inv = 1.f / (float)s;
-    }
-    if (MODE != LG_LOGP && dz && live) {
+    for (int q = 0; q < SUB; ++q) {
+      const long long row = first + q * TEAMS + team;
+      w[q] = Row{row, 0, 0, false, false};
+      if (row < R.rows) w[q] = lg_row(R, row);                 // (all lanes take part in the exchanges below)
+      in[q] = w[q].counts && !w[q].bad;
+      const T *__restrict__ z = (const T *)R.z + row * R.ld;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int j = (k * LANES + lane) * LG_VEC;
-        if (j >= V) continue;
-        if (in && c == c) lg_gradient(dz + j, V - j, v[k], lg_base(M), -c * inv, c, j, (int)w.y);
-        else lg_fill(dz + j, V - j, c);
+        v[q][k] = lg_load(z + j, in[q] ? V - j : 0);
+      }
+      zy[q] = MODE != LG_BACK && in[q] ? (float)z[w[q].y] : 0.f;
+      if (lane == q) mine = w[q];
+    }
+    float M[SUB], inv[SUB], c[SUB];
+    if (MODE == LG_BACK) {
+#pragma unroll
+      for (int q = 0; q < SUB; ++q) {
+        c[q] = 0.f; M[q] = 0.f; inv[q] = 0.f;
+        if (w[q].counts) c[q] = w[q].bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w[q].owner : w[q].at] * up;
+        if (in[q]) { const float2 st = O.stat[w[q].at]; M[q] = st.x; inv[q] = st.y; }
+      }
+    } else {
+      const bool live = lane < SUB && mine.counts && !mine.bad;
+      Pre pre{1.0, 0.f, 0.f, 0.f};
+      if (MODE == LG_POLICY && live) pre = lg_pre(R, P, mine);
+      float my_m = 0.f, my_zy = 0.f;
+      double my_s = 1.0;
+#pragma unroll
+      for (int q = 0; q < SUB; ++q) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) { m = lg_top(v[q][k], m); if (SUB * NV > 1) lg_forget(v[q][k]); }
+        M[q] = lg_lanes_max<LANES>(m);
+        double s = 0.0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) { s += lg_sum(v[q][k], lg_base(M[q])); if (SUB * NV > 1) lg_forget(v[q][k]); }
+        s = lg_lanes_sum<LANES>(s);
+        inv[q] = 1.f / (float)s;
+        if (lane == q) { my_m = M[q]; my_s = s; my_zy = zy[q]; }
+      }
+      float my_c = 0.f;
+      if (live) my_c = lg_finish(P, O, mine.at, pre, my_zy, my_m, my_s, true, MODE == LG_POLICY, add);
+      else if (lane < SUB && mine.at < R.rows) my_c = lg_void(R, P, O, mine, true, MODE == LG_POLICY, add);
+#pragma unroll
+      for (int q = 0; q < SUB; ++q) c[q] = __shfl(my_c, q, LANES);
+    }
+    if (MODE != LG_LOGP && O.dz) {
+#pragma unroll
+      for (int q = 0; q < SUB; ++q) {
+        if (w[q].at >= R.rows) continue;
+        T *__restrict__ dz = (T *)O.dz + w[q].at * V;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int j = (k * LANES + lane) * LG_VEC;
+          if (j >= V) continue;
+          if (in[q] && c[q] == c[q]) lg_gradient(dz + j, V - j, v[q][k], lg_base(M[q]), -c[q] * inv[q], c[q], j, (int)w[q].y);
+          else lg_fill(dz + j, V - j, c[q]);
+        }
       }
     }
   }
   if (MODE == LG_POLICY) lg_partial<256>(P, add, (int)blockIdx.x);
 }
 
+// The logits z[0, left) of a workgroup's THREADS threads, 8 to a thread and step.  The first `full` steps are whole: their loads ask no
+// question and leave in one go, from an address that the workgroup shares and a thread's offset in it.  The step behind them, where each
+// thread asks, is `tail`.
+template <typename T, int THREADS>
+__device__ __forceinline__ void lg_step(const T *__restrict__ z, int k, unsigned off, bool there, Vec<T> &v) {
+  if (there) __builtin_memcpy(&v, (const char *)(z + (long long)k * (THREADS * LG_VEC)) + off, sizeof(v));
+  else __builtin_memset(&v, 0, sizeof(v));                   // (never looked at; left undefined, it would be carried from row to row)
+}
+template <typename T, int THREADS>
+__device__ __forceinline__ void lg_step_out(T *__restrict__ dz, int k, unsigned off, int tid, const Vec<T> &v, float base, float scale, float c, int y) {
+  T *at = (T *)((char *)(dz + (long long)k * (THREADS * LG_VEC)) + off);
+  lg_gradient(at, LG_VEC, v, base, scale, c, (k * THREADS + tid) * LG_VEC, y);
+}
+
 // Long rows, one workgroup each, LDS for what its waves tell each other.  HELD (the policy loss): the row stays in registers between its
-// sum and its gradient, NV vectors of 8 per thread.  Otherwise chunks of NV vectors are taken in turn: their loads are all in flight
-// before the first is used, and the running maximum is corrected once per chunk.
-template <typename T, int MODE, int THREADS, int NV, bool HELD>
-__global__ void __launch_bounds__(THREADS)
+// sum and its gradient, at most NV steps of 8 logits per thread and a tail.  Otherwise chunks of NV steps are taken in turn: their loads
+// are all in flight before the first is used, and the running maximum is corrected once per chunk.
+// (WAVES per SIMD bound the registers: left alone, the compiler interleaves the steps until two waves are all that fits)
+template <typename T, int MODE, int THREADS, int NV, bool HELD, int WAVES>
+__global__ void __launch_bounds__(THREADS, WAVES)
 long_kernel(Rows R, Policy P, Outs O) {
-  constexpr int W = THREADS / 64;
+  constexpr int W = THREADS / 64, STEP = THREADS * LG_VEC;
   __shared__ float red_m[2][W];
   __shared__ double red_s[2][W];
   __shared__ float red_c[2];
   const int tid = (int)threadIdx.x, wave = tid >> 6, V = R.classes;
+  const unsigned off = (unsigned)tid * (LG_VEC * sizeof(T));
+  const int full = V / STEP, last = full * STEP + tid * LG_VEC;          // whole steps, and the thread's first logit behind them
   double add[3] = {0.0, 0.0, 0.0};
   int turn = 0;                       // scratch of two rows in turn: a row's last reader is a barrier ahead of the next but one's writer
   for (long long row = blockIdx.x; row < R.rows; row += gridDim.x) {
@@ -333,23 +390,29 @@ long_kernel(Rows R, Policy P, Outs O) {
     if (!w.counts || w.bad) {
       const float fill = lg_void(R, P, O, w, tid == 0, MODE == LG_POLICY, add);
       if (MODE == LG_POLICY && dz)
-        for (int j = tid * LG_VEC; j < V; j += THREADS * LG_VEC) lg_fill(dz + j, V - j, fill);
+        for (int j = tid * LG_VEC; j < V; j += STEP) lg_fill(dz + j, V - j, fill);
       continue;
     }
     turn ^= 1;
-    Vec<T> v[NV];
+    Vec<T> v[NV], tail;
     float m = -INFINITY, M;
     double s = 0.0;
+    Pre pre{1.0, 0.f, 0.f, 0.f};
     const float zy = (float)z[w.y];
+    if (MODE == LG_POLICY && wave == 0) pre = lg_pre(R, P, w);
     if (HELD) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) v[k] = lg_load(z + (k * THREADS + tid) * LG_VEC, V - (k * THREADS + tid) * LG_VEC);
+      for (int k = 0; k < NV; ++k) lg_step<T, THREADS>(z, k, off, k < full, v[k]);
+      tail = lg_load(z + last, V - last);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) { m = lg_top(v[k], m); lg_forget(v[k]); }
+      for (int k = 0; k < NV; ++k) if (k < full) { m = lg_top(v[k], m); lg_forget(v[k]); }
+      m = lg_top(tail, m);
+      lg_forget(tail);
     } else {
-      for (int j0 = 0; j0 < V; j0 += THREADS * LG_VEC * NV) {
+      int k0 = 0;
+      for (; k0 + NV <= full; k0 += NV) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) { const int j = j0 + (k * THREADS + tid) * LG_VEC; v[k] = lg_load(z + (j < V ? j : 0), V - j); }
+        for (int k = 0; k < NV; ++k) lg_step<T, THREADS>(z, k0 + k, off, true, v[k]);
         float top = m;
 #pragma unroll
         for (int k = 0; k < NV; ++k) top = lg_top(v[k], top);
@@ -357,6 +420,16 @@ long_kernel(Rows R, Policy P, Outs O) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) s += lg_sum(v[k], lg_base(m));
       }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) lg_step<T, THREADS>(z, k0 + k, off, k0 + k < full, v[k]);
+      tail = lg_load(z + last, V - last);
+      float top = lg_top(tail, m);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) if (k0 + k < full) top = lg_top(v[k], top);
+      if (top > m) { s *= (double)lg_exp(m - top); m = top; }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) if (k0 + k < full) s += lg_sum(v[k], lg_base(m));
+      s += lg_sum(tail, lg_base(m));
     }
     M = lg_lanes_max<64>(m);
     if ((tid & 63) == 0) red_m[turn][wave] = M;
@@ -364,10 +437,12 @@ long_kernel(Rows R, Policy P, Outs O) {
     M = red_m[turn][0];
 #pragma unroll
     for (int k = 1; k < W; ++k) M = fmaxf(M, red_m[turn][k]);
-    float base = lg_base(M);
+    const float base = lg_base(M);
     if (HELD) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) { s += lg_sum(v[k], base); lg_forget(v[k]); }
+      for (int k = 0; k < NV; ++k) if (k < full) { s += lg_sum(v[k], base); lg_forget(v[k]); }
+      s += lg_sum(tail, base);
+      lg_forget(tail);
     } else if (m != -INFINITY) s *= (double)lg_exp(m - base);
     s = lg_lanes_sum<64>(s);
     if ((tid & 63) == 0) red_s[turn][wave] = s;
@@ -377,27 +452,36 @@ long_kernel(Rows R, Policy P, Outs O) {
     for (int k = 1; k < W; ++k) s += red_s[turn][k];
     float c = 0.f;
     if (wave == 0) {
-      c = lg_finish<T>(R, P, O, w, zy, M, s, tid == 0, MODE == LG_POLICY, add);
+      c = lg_finish(P, O, row, pre, zy, M, s, tid == 0, MODE == LG_POLICY, add);
       if (tid == 0) red_c[turn] = c;
     }
     if (MODE == LG_POLICY && dz) {
       __syncthreads();
       c = red_c[turn];
       const float scale = -c * (1.f / (float)s);
+      const int y = (int)w.y;
+      if (c != c) {
+        for (int j = tid * LG_VEC; j < V; j += STEP) lg_fill(dz + j, V - j, c);
+        continue;
+      }
       if (HELD) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int j = (k * THREADS + tid) * LG_VEC;
-          if (j >= V) continue;
-          if (c == c) lg_gradient(dz + j, V - j, v[k], base, scale, c, j, (int)w.y);
-          else lg_fill(dz + j, V - j, c);
-        }
+        for (int k = 0; k < NV; ++k) if (k < full) lg_step_out<T, THREADS>(dz, k, off, tid, v[k], base, scale, c, y);
       } else {
-        for (int j = tid * LG_VEC; j < V; j += THREADS * LG_VEC) {
-          if (c == c) lg_gradient(dz + j, V - j, lg_load(z + j, V - j), base, scale, c, j, (int)w.y);
-          else lg_fill(dz + j, V - j, c);
+        int k0 = 0;
+        for (; k0 + NV <= full; k0 += NV) {
+#pragma unroll
+          for (int k = 0; k < NV; ++k) lg_step<T, THREADS>(z, k0 + k, off, true, v[k]);
+#pragma unroll
+          for (int k = 0; k < NV; ++k) lg_step_out<T, THREADS>(dz, k0 + k, off, tid, v[k], base, scale, c, y);
         }
+        for (; k0 < full; ++k0) {
+          lg_step<T, THREADS>(z, k0, off, true, v[0]);
+          lg_step_out<T, THREADS>(dz, k0, off, tid, v[0], base, scale, c, y);
+        }
+        tail = lg_load(z + last, V - last);
       }
+      if (last < V) lg_gradient(dz + last, V - last, tail, base, scale, c, last, y);
     }
   }
   if (MODE == LG_POLICY) lg_partial<THREADS>(P, add, (int)blockIdx.x);
@@ -405,34 +489,35 @@ long_kernel(Rows R, Policy P, Outs O) {
 
 // backward pass of long rows: a workgroup takes 256 * 8 * NV logits of a row at a time, whatever row they are of
 template <typename T, int NV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 7)
 long_back_kernel(Rows R, Outs O, int parts) {
+  constexpr int STEP = 256 * LG_VEC;
   const float up = O.up ? *O.up : 1.f;
   if (O.skip_unit && up == 1.f) return;
   const int tid = (int)threadIdx.x, V = R.classes;
-  const long long all = R.rows * parts;
-  for (long long b = blockIdx.x; b < all; b += gridDim.x) {
-    const long long row = b / parts;
-    const int j0 = (int)(b - row * parts) * (256 * LG_VEC * NV);
+  const unsigned off = (unsigned)tid * (LG_VEC * sizeof(T));
+  for (long long row = blockIdx.y; row < R.rows; row += gridDim.y)
+  for (int part = blockIdx.x; part < parts; part += gridDim.x) {
+    const int j0 = part * (STEP * NV);
     const Row w = lg_row(R, row);
-    const T *__restrict__ z = (const T *)R.z + row * R.ld;
-    T *__restrict__ dz = (T *)O.dz + row * V;
+    const T *__restrict__ z = (const T *)R.z + row * R.ld + j0;
+    T *__restrict__ dz = (T *)O.dz + row * V + j0;
+    const int left = V - j0, full = left / STEP < NV ? left / STEP : NV, y = (int)w.y - j0;
     float c = 0.f;
     if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w.owner : row] * up;
     if (c == 0.f || c != c) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; if (j < V) lg_fill(dz + j, V - j, c); }
+      for (int j = tid * LG_VEC; j < left && j < STEP * NV; j += STEP) lg_fill(dz + j, left - j, c);
       continue;
     }
-    const float2 st = O.stat[row];
     Vec<T> v[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; v[k] = lg_load(z + (j < V ? j : 0), V - j); }
+    for (int k = 0; k < NV; ++k) lg_step<T, 256>(z, k, off, k < full, v[k]);
+    const float2 st = O.stat[row];
+    const float base = lg_base(st.x), scale = -c * st.y;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int j = j0 + (k * 256 + tid) * LG_VEC;
-      if (j < V) lg_gradient(dz + j, V - j, v[k], lg_base(st.x), -c * st.y, c, j, (int)w.y);
-    }
+    for (int k = 0; k < NV; ++k) if (k < full) lg_step_out<T, 256>(dz, k, off, tid, v[k], base, scale, c, y);
+    const int last = full * STEP + tid * LG_VEC;
+    if (full < NV && last < left) lg_gradient(dz + last, left - last, lg_load(z + last, left - last), base, scale, c, last, y);
   }
 }
 
@@ -453,7 +538,7 @@ part_kernel(Rows R, int parts, int piece, float *__restrict__ part_m, double *__
   for (int j0 = from; j0 < to; j0 += 256 * LG_VEC * NV) {
     Vec<T> v[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; v[k] = lg_load(z + (j < to ? j : 0), to - j); }
+    for (int k = 0; k < NV; ++k) { const int j = j0 + (k * 256 + tid) * LG_VEC; v[k] = lg_load(z + j, to - j); }
     float top = m;
 #pragma unroll
     for (int k = 0; k < NV; ++k) top = lg_top(v[k], top);
@@ -485,12 +570,14 @@ join_kernel(Rows R, Policy P, Outs O, int parts, const float *__restrict__ part_
   if (!w.counts || w.bad) lg_void(R, P, O, w, lane == 0, MODE == LG_POLICY, add);
   else {
     const float zy = (float)((const T *)R.z + row * R.ld)[w.y];
+    Pre pre{1.0, 0.f, 0.f, 0.f};
+    if (MODE == LG_POLICY) pre = lg_pre(R, P, w);
     const float m = lane < parts ? part_m[row * parts + lane] : -INFINITY;
     const float M = lg_lanes_max<64>(m);
     double s = lane < parts ? part_s[row * parts + lane] : 0.0;
     if (m != -INFINITY) s *= (double)lg_exp(m - lg_base(M));
     s = lg_lanes_sum<64>(s);
-    lg_finish<T>(R, P, O, w, zy, M, s, lane == 0, MODE == LG_POLICY, add);
+    lg_finish(P, O, row, pre, zy, M, s, lane == 0, MODE == LG_POLICY, add);
   }
   if (MODE == LG_POLICY) lg_partial<64>(P, add, (int)blockIdx.x);
 }
@@ -583,7 +670,7 @@ Rows rows_of(const rs_logits *l) {
 }
 
 constexpr int LG_GRID = 2048;             // 8 workgroups of 256 threads on each of 256 CUs
-constexpr int LG_SHORT = 2048;            // classes of the longest row that a wave holds
+constexpr int LG_SHORT = 4096;            // classes of the longest row that a wave holds
 constexpr int LG_FEW = 256, LG_PARTS = 64;
 static_assert(LG_PARTS == RS_LOGITS_PARTS && LG_FEW == RS_LOGITS_FEW_ROWS, "room of the callers' scratch");
 
@@ -599,7 +686,7 @@ int parts_of(const rs_logits *l) {
 template <typename T, int MODE>
 int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &O, hipStream_t st) {
   const int V = R.classes;
-#define LG_RUN_SHORT(L, N) { const int g = lesser((R.rows + 256 / L - 1) / (256 / L), LG_GRID); hipLaunchKernelGGL((short_kernel<T, MODE, L, N>), dim3(g), dim3(256), 0, st, R, P, O); return g; }
+#define LG_RUN_SHORT(L, N) { const int sub = MODE != LG_POLICY ? 1 : L < 8 / N ? L : (8 / N), per = 256 / L * sub, g = lesser((R.rows + per - 1) / per, LG_GRID); hipLaunchKernelGGL((short_kernel<T, MODE, L, N>), dim3(g), dim3(256), 0, st, R, P, O); return g; }
   if (V <= 16) LG_RUN_SHORT(2, 1)
   if (V <= 32) LG_RUN_SHORT(4, 1)
   if (V <= 64) LG_RUN_SHORT(8, 1)
@@ -607,24 +694,30 @@ int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &
   if (V <= 256) LG_RUN_SHORT(32, 1)
   if (V <= 512) LG_RUN_SHORT(64, 1)
   if (V <= 1024) LG_RUN_SHORT(64, 2)
-  if (V <= LG_SHORT) LG_RUN_SHORT(64, 4)
+  if (V <= 2048) LG_RUN_SHORT(64, 4)
+  if (V <= LG_SHORT) LG_RUN_SHORT(64, 8)
 #undef LG_RUN_SHORT
   if constexpr (MODE == LG_BACK) {
     constexpr int NV = 4;
-    const int parts = (V + 256 * LG_VEC * NV - 1) / (256 * LG_VEC * NV), g = lesser(R.rows * parts, 2 * LG_GRID);
-    hipLaunchKernelGGL((long_back_kernel<T, NV>), dim3(g), dim3(256), 0, st, R, O, parts);
-    return g;
+    const int parts = (V + 256 * LG_VEC * NV - 1) / (256 * LG_VEC * NV), across = lesser(parts, LG_GRID);
+    hipLaunchKernelGGL((long_back_kernel<T, NV>), dim3(across, lesser(R.rows, 2 * LG_GRID / across)), dim3(256), 0, st, R, O, parts);
+    return 0;
   } else {
-#define LG_RUN_LONG(TH, N, H) { const int g = lesser(R.rows, LG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
+#define LG_RUN_LONG(TH, N, H, WV) { const int g = lesser(R.rows, LG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H, WV>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
     if constexpr (MODE == LG_POLICY) {       // (without a gradient too: the loss has the same bits either way)
-      if (V <= 4096) LG_RUN_LONG(256, 2, true)
-      if (V <= 8192) LG_RUN_LONG(256, 4, true)
-      if (V <= 16384) LG_RUN_LONG(512, 4, true)
-      if (V <= 32768) LG_RUN_LONG(1024, 4, true)
-      if (V <= 65536) LG_RUN_LONG(1024, 8, true)
-      if constexpr (sizeof(T) == 2) { if (V <= 131072) LG_RUN_LONG(1024, 16, true) }
+      constexpr int K = sizeof(T) / 2;       // 8 logits: 4 or 8 registers of a thread
+      if (V < 10240) LG_RUN_LONG(256, 4, true, K == 1 ? 5 : 4)
+      if (V < 18432) LG_RUN_LONG(256, 8, true, K == 1 ? 4 : 3)
+      if (V < 34816) LG_RUN_LONG(256, 16, true, K == 1 ? 3 : 2)
+      if constexpr (K == 1) {
+        if (V < 51200) LG_RUN_LONG(256, 24, true, 3)
+        if (V < 67584) LG_RUN_LONG(256, 32, true, 2)
+        if (V < 135168) LG_RUN_LONG(512, 32, true, 2)
+      } else {
+        if (V < 69632) LG_RUN_LONG(512, 16, true, 2)
+      }
     }
-    LG_RUN_LONG(256, 4, false)
+    LG_RUN_LONG(256, 4, false, MODE == LG_POLICY ? 4 : 6)
 #undef LG_RUN_LONG
   }
 }
