@@ -85,37 +85,58 @@ __device__ __forceinline__ unsigned aw_field(float x) {
   return f == 255u ? 0u : f;
 }
 
-__device__ __forceinline__ float aw_master(unsigned short p, short low) {
-  const unsigned a = p & 0x7FFFu;
-  // +-0 and infinity never carry a remainder of this sign: such a parameter was written from outside, and its word would wrap to a NaN
-  const int l = (a == 0u && low < 0) || (a >= 0x7F80u && low > 0) ? 0 : (int)low;
-  return __uint_as_float(((unsigned)p << 16) + (unsigned)l);
+// (a word that is no number without its parameter being none: +-0 and infinity never carry a remainder of that sign, such a parameter
+// was written from outside, and its remainder is dropped)
+__device__ __forceinline__ float aw_master(unsigned p_high, int low) {
+  const float x = __uint_as_float(p_high + (unsigned)low);
+  return x != x ? __uint_as_float(p_high) : x;
 }
-__device__ __forceinline__ void aw_split(float x, unsigned short &p, short &low) {
-  const unsigned b = __float_as_uint(x);
-  const bool nan = (b & 0x7FFFFFFFu) > 0x7F800000u;
-  p = nan ? (unsigned short)0x7FC0u : (unsigned short)((b + 0x8000u) >> 16);
-  low = nan ? (short)0 : (short)(b - ((unsigned)p << 16));
-}
+// the master's word as it is kept: its upper half rounded is the parameter, its lower half, as a signed number, the remainder
+__device__ __forceinline__ unsigned aw_word(float x) { return x != x ? 0x7FC00000u : __float_as_uint(x); }
 
 template <bool BF16> struct AwType { typedef float T; };
 template <> struct AwType<true> { typedef unsigned short T; };
 
-// four consecutive elements; `left` of them exist.  The address is aligned to the element only: global loads of this device need no more.
-template <typename T> struct Four { T x[4]; };
+// four consecutive elements as the words they come in; `left` of them exist.  The address is aligned to the element only: global loads and
+// stores of this device need no more.
+template <typename T> struct Four { unsigned w[sizeof(T)]; };
 template <typename T>
 __device__ __forceinline__ Four<T> aw_load(const T *p, long long left) {
   Four<T> r;
   if (left >= 4) { __builtin_memcpy(&r, p, sizeof(r)); return r; }
+  T x[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r.x[i] = i < left ? p[i] : T(0);
+  for (int i = 0; i < 4; ++i) x[i] = i < left ? p[i] : T(0);
+  __builtin_memcpy(&r, x, sizeof(r));
   return r;
 }
 template <typename T>
 __device__ __forceinline__ void aw_store(T *p, const Four<T> &r, long long left) {
   if (left >= 4) { __builtin_memcpy(p, &r, sizeof(r)); return; }
+  T x[4];
+  __builtin_memcpy(x, &r, sizeof(r));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) if (i < left) p[i] = r.x[i];
+  for (int i = 0; i < 4; ++i) if (i < left) p[i] = x[i];
+}
+__device__ __forceinline__ float aw_get(const Four<float> &r, int i) { return __uint_as_float(r.w[i]); }
+__device__ __forceinline__ unsigned aw_high(const Four<unsigned short> &r, int i) { return i & 1 ? r.w[i >> 1] & 0xFFFF0000u : r.w[i >> 1] << 16; }
+__device__ __forceinline__ float aw_get(const Four<unsigned short> &r, int i) { return __uint_as_float(aw_high(r, i)); }      // bf16
+__device__ __forceinline__ int aw_get(const Four<short> &r, int i) { return i & 1 ? (int)r.w[i >> 1] >> 16 : (int)(r.w[i >> 1] << 16) >> 16; }
+__device__ __forceinline__ unsigned aw_get(const Four<unsigned char> &r, int i) { return (r.w[0] >> (8 * i)) & 255u; }
+// the larger of two pairs of 16-bit numbers, each half by itself, over a wave
+__device__ __forceinline__ unsigned aw_pair_max(unsigned a, unsigned b) {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+}
+__device__ __forceinline__ unsigned aw_wave_pair_max(unsigned v) {
+  v = aw_pair_max(v, rs_dpp<RS_DPP_QUAD_XOR1>(v));
+  v = aw_pair_max(v, rs_dpp<RS_DPP_QUAD_XOR2>(v));
+  v = aw_pair_max(v, rs_dpp<RS_DPP_ROW_HALF_MIRROR>(v));
+  v = aw_pair_max(v, rs_dpp<RS_DPP_ROW_MIRROR>(v));
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = aw_pair_max((unsigned)r[0], (unsigned)r[1]);
+  auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return rs_uniform((int)aw_pair_max((unsigned)s[0], (unsigned)s[1]));
 }
 
 // max(1, ...) of torch.nn.utils.clip_grad_norm_: max_norm / (norm + 1e-6), at most 1; a norm that is not a number stays one
@@ -134,6 +155,99 @@ __device__ __forceinline__ float aw_clip(const double *partial, int n, float max
   return c > 1.f ? 1.f : c;
 }
 
+// what a launch's elements share, and what a tensor's do
+struct AwShared {
+  float eps, decay, omb1, b2, omb2, clip;
+  float step_size, inv_bc2;
+  unsigned key;
+};
+
+// N blocks of a wave from element `b` of a tensor on.  WHOLE: all of their elements exist, so the loads ask no question and leave in one go.
+template <bool BF16, int BITS, int N, bool WHOLE>
+struct AwBlocks {
+  typedef typename AwType<BF16>::T PT;
+  Four<PT> p[N], g[N];
+  Four<short> low[N];
+  Four<float> m[N], v[N];
+  Four<unsigned char> mc[N], vc[N];
+  int em[N], ev[N];
+
+  __device__ __forceinline__ void load(const AwArgs &A, const PT *__restrict__ pp, const PT *__restrict__ gp, long long at, long long b, int lane, long long n) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const long long e = b + u * AW_BLOCK + lane * 4, left = WHOLE ? 4 : n - e;
+      p[u] = aw_load(pp + e, left);
+      g[u] = aw_load(gp + e, left);
+      if constexpr (BF16) low[u] = aw_load((const short *)A.low + at + e, 4);
+      if constexpr (BITS == 32) {         // (the flat buffers have the block's tail, as zeros)
+        m[u] = aw_load((const float *)A.m + at + e, 4);
+        v[u] = aw_load((const float *)A.v + at + e, 4);
+      } else {
+        mc[u] = aw_load((const unsigned char *)A.m + at + e, 4);
+        vc[u] = aw_load((const unsigned char *)A.v + at + e, 4);
+        em[u] = A.me[(at + b + u * AW_BLOCK) >> 8];
+        ev[u] = A.ve[(at + b + u * AW_BLOCK) >> 8];
+      }
+    }
+  }
+  __device__ __forceinline__ void update(const AwArgs &A, const AwShared &S, PT *__restrict__ pp, long long at, long long b, int lane, long long n) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const long long e = b + u * AW_BLOCK + lane * 4, left = WHOLE ? 4 : n - e;
+      const long long block = (at + b + u * AW_BLOCK) >> 8;
+      unsigned fields = 0u, word[4];
+      float mi[4], vi[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x, gi = aw_get(g[u], i);
+        if constexpr (BF16) x = aw_master(aw_high(p[u], i), aw_get(low[u], i)); else x = aw_get(p[u], i);
+        if constexpr (BITS == 8) { mi[i] = aw_decode_m(aw_get(mc[u], i), em[u]); vi[i] = aw_decode_v(aw_get(vc[u], i), ev[u]); }
+        else { mi[i] = aw_get(m[u], i); vi[i] = aw_get(v[u], i); }
+        gi *= S.clip;
+        mi[i] = rs_fma(gi - mi[i], S.omb1, mi[i]);
+        vi[i] = rs_fma(S.omb2 * gi, gi, vi[i] * S.b2);
+        // The device's own root and reciprocal, each off by one unit: the correctly rounded ones are 25 instructions for an error that lr
+        // scales away.  The root takes denormals as zero, so v is raised to the smallest normal number (1e-19 beside eps).
+        const float root = __builtin_amdgcn_sqrtf(fmaxf(vi[i], 1.17549435e-38f));
+        x = rs_fma(-S.step_size, mi[i] * __builtin_amdgcn_rcpf(rs_fma(root, S.inv_bc2, S.eps)), x * S.decay);
+        if (!WHOLE && i >= left) mi[i] = vi[i] = x = 0.f;
+        if constexpr (BF16) word[i] = aw_word(x); else p[u].w[i] = __float_as_uint(x);
+        if constexpr (BITS == 8) fields = aw_pair_max(fields, aw_field(mi[i]) << 16 | aw_field(vi[i]));
+        else { m[u].w[i] = __float_as_uint(mi[i]); v[u].w[i] = __float_as_uint(vi[i]); }
+      }
+      if constexpr (BF16) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          p[u].w[i] = ((word[2 * i + 1] + 0x8000u) & 0xFFFF0000u) | ((word[2 * i] + 0x8000u) >> 16);
+          low[u].w[i] = (word[2 * i + 1] << 16) | (word[2 * i] & 0xFFFFu);
+        }
+      }
+      aw_store(pp + e, p[u], left);
+      if constexpr (BF16) aw_store(A.low + at + e, low[u], 4);
+      if constexpr (BITS == 32) {
+        aw_store((float *)A.m + at + e, m[u], 4);
+        aw_store((float *)A.v + at + e, v[u], 4);
+      } else {
+        fields = aw_wave_pair_max(fields);
+        const int fm = (int)(fields >> 16), fv = (int)(fields & 255u);
+        const unsigned k = aw_mix(S.key + (unsigned)block) + (unsigned)(lane * 4) * AW_PHI;
+        unsigned a = 0u, c = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned r = aw_mix(k + i * AW_PHI);
+          a |= aw_encode_m(mi[i], fm, r >> 16) << (8 * i);
+          c |= aw_encode_v(vi[i], fv, r & 0xFFFFu) << (8 * i);
+        }
+        mc[u].w[0] = a;
+        vc[u].w[0] = c;
+        aw_store((unsigned char *)A.m + at + e, mc[u], 4);
+        aw_store((unsigned char *)A.v + at + e, vc[u], 4);
+        if (lane == 0) { A.me[block] = (unsigned char)fm; A.ve[block] = (unsigned char)fv; }
+      }
+    }
+  }
+};
+
 template <bool BF16, int BITS>
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_kernel(AwTable T, AwArgs A) {
@@ -144,15 +258,12 @@ adamw_kernel(AwTable T, AwArgs A) {
     lr = A.hyper_dev[0]; beta1 = A.hyper_dev[1]; beta2 = A.hyper_dev[2]; eps64 = A.hyper_dev[3]; wd = A.hyper_dev[4];
     lnb1 = A.hyper_dev[5]; lnb2 = A.hyper_dev[6];
   }
-  const float eps = (float)eps64, decay = (float)(1.0 - lr * wd);
-  const float omb1 = (float)(1.0 - beta1), b2 = (float)beta2, omb2 = (float)(1.0 - beta2);
-  const float clip = A.partial ? aw_clip(A.partial, A.npartial, A.max_norm, A.norm, red) : 1.f;
+  AwShared S{(float)eps64, (float)(1.0 - lr * wd), (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), 1.f, 0.f, 1.f, 0u};
+  if (A.partial) S.clip = aw_clip(A.partial, A.npartial, A.max_norm, A.norm, red);
   const int wave = rs_uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int chunks = T.blk_end[T.count - 1];
 
   int ti = 0, seen = -1;
-  float step_size = 0.f, inv_bc2 = 1.f;
-  unsigned key = 0u;
   for (int c = (int)blockIdx.x; c < chunks; c += (int)gridDim.x) {
     // the tensor of this chunk: the first whose running count exceeds c, by bisection above the last one (chunks only grow)
     int lo = ti, hi = T.count - 1;
@@ -161,82 +272,27 @@ adamw_kernel(AwTable T, AwArgs A) {
       if (c >= T.blk_end[mid]) lo = mid + 1; else hi = mid;
     }
     ti = lo;
+    const long long n = T.n[ti], at = T.at[ti];
+    const long long b = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK + wave * (AW_BLOCK * AW_UNROLL);
+    PT *__restrict__ p = (PT *)T.p[ti];
+    const PT *__restrict__ g = (const PT *)T.g[ti];
+    const bool whole = b + AW_BLOCK * AW_UNROLL <= n;
+    AwBlocks<BF16, BITS, AW_UNROLL, true> W;
+    if (whole) W.load(A, p, g, at, b, lane, n);               // (in front of the step count, which the loads do not need)
     if (ti != seen) {
       seen = ti;
       const int t = A.step[T.slot[ti]] + 1;
       // 1 - beta^t as -expm1(t ln beta): fp32 loses nothing where beta^t is near 1
-      step_size = (float)(lr / (double)-expm1f((float)(lnb1 * t)));
-      inv_bc2 = 1.f / sqrtf(-expm1f((float)(lnb2 * t)));
-      key = aw_mix(A.seed + (unsigned)t * AW_PHI);
+      S.step_size = (float)(lr / (double)-expm1f((float)(lnb1 * t)));
+      S.inv_bc2 = 1.f / sqrtf(-expm1f((float)(lnb2 * t)));
+      S.key = aw_mix(A.seed + (unsigned)t * AW_PHI);
     }
-    const long long n = T.n[ti], at = T.at[ti];
-    const long long base = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK + wave * (AW_BLOCK * AW_UNROLL);
-    PT *__restrict__ p = (PT *)T.p[ti];
-    const PT *__restrict__ g = (const PT *)T.g[ti];
-    Four<PT> pv[AW_UNROLL], gv[AW_UNROLL];
-    Four<short> lv[AW_UNROLL];
-    Four<float> mv[AW_UNROLL], vv[AW_UNROLL];
-    Four<unsigned char> mc[AW_UNROLL], vc[AW_UNROLL];
-    int em[AW_UNROLL], ev[AW_UNROLL];
-#pragma unroll
-    for (int u = 0; u < AW_UNROLL; ++u) {
-      const long long b = base + u * AW_BLOCK, e = b + lane * 4, left = n - e;
-      if (b >= n) continue;
-      pv[u] = aw_load(p + e, left);
-      gv[u] = aw_load(g + e, left);
-      if constexpr (BF16) lv[u] = aw_load((const short *)A.low + at + e, 4);
-      if constexpr (BITS == 32) {         // (the flat buffers have the block's tail, as zeros)
-        mv[u] = aw_load((const float *)A.m + at + e, 4);
-        vv[u] = aw_load((const float *)A.v + at + e, 4);
-      } else {
-        mc[u] = aw_load((const unsigned char *)A.m + at + e, 4);
-        vc[u] = aw_load((const unsigned char *)A.v + at + e, 4);
-        em[u] = A.me[(at + b) >> 8];
-        ev[u] = A.ve[(at + b) >> 8];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < AW_UNROLL; ++u) {
-      const long long b = base + u * AW_BLOCK, e = b + lane * 4, left = n - e;
-      if (b >= n) continue;
-      unsigned fm = 0u, fv = 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x, gi;
-        if constexpr (BF16) {
-          x = aw_master(pv[u].x[i], lv[u].x[i]);
-          gi = __uint_as_float((unsigned)gv[u].x[i] << 16);
-        } else { x = pv[u].x[i]; gi = gv[u].x[i]; }
-        if constexpr (BITS == 8) { mv[u].x[i] = aw_decode_m(mc[u].x[i], em[u]); vv[u].x[i] = aw_decode_v(vc[u].x[i], ev[u]); }
-        gi *= clip;
-        const float m = rs_fma(gi - mv[u].x[i], omb1, mv[u].x[i]);
-        const float v = rs_fma(omb2 * gi, gi, vv[u].x[i] * b2);
-        x = rs_fma(-step_size, m / rs_fma(sqrtf(v), inv_bc2, eps), x * decay);
-        const bool in = i < left;
-        mv[u].x[i] = in ? m : 0.f;
-        vv[u].x[i] = in ? v : 0.f;
-        if constexpr (BF16) aw_split(x, pv[u].x[i], lv[u].x[i]); else pv[u].x[i] = x;
-        if constexpr (BF16) { if (!in) lv[u].x[i] = 0; }
-        if constexpr (BITS == 8) { fm = max(fm, aw_field(mv[u].x[i])); fv = max(fv, aw_field(vv[u].x[i])); }
-      }
-      aw_store(p + e, pv[u], left);
-      if constexpr (BF16) aw_store(A.low + at + e, lv[u], 4);
-      if constexpr (BITS == 32) {
-        aw_store((float *)A.m + at + e, mv[u], 4);
-        aw_store((float *)A.v + at + e, vv[u], 4);
-      } else {
-        fm = rs_wave_max_u32(fm);
-        fv = rs_wave_max_u32(fv);
-        const unsigned k = aw_mix(key + (unsigned)((at + b) >> 8)) + (unsigned)(lane * 4) * AW_PHI;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned r = aw_mix(k + i * AW_PHI);
-          mc[u].x[i] = (unsigned char)aw_encode_m(mv[u].x[i], (int)fm, r >> 16);
-          vc[u].x[i] = (unsigned char)aw_encode_v(vv[u].x[i], (int)fv, r & 0xFFFFu);
-        }
-        aw_store((unsigned char *)A.m + at + e, mc[u], 4);
-        aw_store((unsigned char *)A.v + at + e, vc[u], 4);
-        if (lane == 0) { A.me[(at + b) >> 8] = (unsigned char)fm; A.ve[(at + b) >> 8] = (unsigned char)fv; }
+    if (whole) W.update(A, S, p, at, b, lane, n);
+    else {
+      for (int u = 0; u < AW_UNROLL && b + u * AW_BLOCK < n; ++u) {
+        AwBlocks<BF16, BITS, 1, false> E;
+        E.load(A, p, g, at, b + u * AW_BLOCK, lane, n);
+        E.update(A, S, p, at, b + u * AW_BLOCK, lane, n);
       }
     }
   }
@@ -273,18 +329,23 @@ grad_sq_kernel(AwTable T, double *__restrict__ partial) {
     const long long n = T.n[ti];
     const long long base = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK;
     const PT *__restrict__ g = (const PT *)T.g[ti];
+    constexpr int U = AW_CHUNK / (4 * AW_THREADS);
+    Four<PT> r[U];
+    if (base + AW_CHUNK <= n) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) r[u] = aw_load(g + base + (u * AW_THREADS + (int)threadIdx.x) * 4, 4);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) { const long long e = base + (u * AW_THREADS + (int)threadIdx.x) * 4; r[u] = aw_load(g + e, n - e); }
+    }
     float a = 0.f;
 #pragma unroll
-    for (int u = 0; u < AW_CHUNK / (4 * AW_THREADS); ++u) {
-      const long long e = base + (u * AW_THREADS + (int)threadIdx.x) * 4;
-      const Four<PT> r = aw_load(g + e, n - e);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float x;
-        if constexpr (BF16) x = __uint_as_float((unsigned)r.x[i] << 16); else x = r.x[i];
+        const float x = aw_get(r[u], i);
         a = rs_fma(x, x, a);
       }
-    }
     s += (double)a;
   }
   red[threadIdx.x] = s;
@@ -306,14 +367,14 @@ adamw_pack_kernel(long long blocks, const float *__restrict__ m, const float *__
     const Four<float> x = aw_load(m + e, 4), y = aw_load(v + e, 4);
     unsigned fm = 0u, fv = 0u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { fm = max(fm, aw_field(x.x[i])); fv = max(fv, aw_field(y.x[i])); }
+    for (int i = 0; i < 4; ++i) { fm = max(fm, aw_field(aw_get(x, i))); fv = max(fv, aw_field(aw_get(y, i))); }
     fm = rs_wave_max_u32(fm);
     fv = rs_wave_max_u32(fv);
-    Four<unsigned char> a, c;
+    Four<unsigned char> a{{0u}}, c{{0u}};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {         // to nearest: a dither of one half
-      a.x[i] = (unsigned char)aw_encode_m(x.x[i], (int)fm, 0x8000u);
-      c.x[i] = (unsigned char)aw_encode_v(y.x[i], (int)fv, 0x8000u);
+      a.w[0] |= aw_encode_m(aw_get(x, i), (int)fm, 0x8000u) << (8 * i);
+      c.w[0] |= aw_encode_v(aw_get(y, i), (int)fv, 0x8000u) << (8 * i);
     }
     aw_store(mc + e, a, 4);
     aw_store(vc + e, c, 4);
@@ -322,14 +383,11 @@ adamw_pack_kernel(long long blocks, const float *__restrict__ m, const float *__
 }
 
 __device__ __forceinline__ void aw_out(float *p, const float *x) { __builtin_memcpy(p, x, 16); }
-__device__ __forceinline__ void aw_out(unsigned short *p, const float *x) {      // to bf16, to nearest even (exact for a code's value)
-  Four<unsigned short> r;
+__device__ __forceinline__ void aw_out(__bf16 *p, const float *x) {      // to nearest even: exact for a code's value
+  __bf16 r[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned b = __float_as_uint(x[i]);
-    r.x[i] = (b & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC0u : (unsigned short)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
-  }
-  __builtin_memcpy(p, &r, sizeof(r));
+  for (int i = 0; i < 4; ++i) r[i] = (__bf16)x[i];
+  __builtin_memcpy(p, r, sizeof(r));
 }
 template <typename O>
 __global__ void __launch_bounds__(AW_THREADS)
@@ -342,13 +400,13 @@ adamw_unpack_kernel(long long blocks, const unsigned char *__restrict__ mc, cons
     const int em = me[b], ev = ve[b];
     float x[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = aw_decode_m(a.x[i], em); y[i] = aw_decode_v(c.x[i], ev); }
+    for (int i = 0; i < 4; ++i) { x[i] = aw_decode_m(aw_get(a, i), em); y[i] = aw_decode_v(aw_get(c, i), ev); }
     aw_out(m + e, x);
     aw_out(v + e, y);
   }
 }
 
-// masters of bf16 parameters into a flat fp32 buffer (its tails are left as they are)
+// masters of bf16 parameters into a flat fp32 buffer, zeros up to the next tensor
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_masters_kernel(AwTable T, const short *__restrict__ low, float *__restrict__ out) {
   const int chunks = T.blk_end[T.count - 1];
@@ -366,13 +424,13 @@ adamw_masters_kernel(AwTable T, const short *__restrict__ low, float *__restrict
 #pragma unroll
     for (int u = 0; u < AW_CHUNK / (4 * AW_THREADS); ++u) {
       const long long e = base + (u * AW_THREADS + (int)threadIdx.x) * 4, left = n - e;
-      if (left <= 0) continue;
+      if (e >= (n + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK) continue;
       const Four<unsigned short> r = aw_load(p + e, left);
       const Four<short> l = aw_load(low + at + e, 4);
       Four<float> x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x.x[i] = aw_master(r.x[i], l.x[i]);
-      aw_store(out + at + e, x, left);
+      for (int i = 0; i < 4; ++i) x.w[i] = i < left ? __float_as_uint(aw_master(aw_high(r, i), aw_get(l, i))) : 0u;
+      aw_store(out + at + e, x, 4);
     }
   }
 }
@@ -470,7 +528,7 @@ extern "C" int rs_adamw_unpack(long long n, const unsigned char *mc, const unsig
   RS_REQUIRE(m && v && mc && vc && me && ve, "rs_adamw_unpack: null pointer");
   const long long blocks = n / AW_BLOCK, wgs = (blocks + 3) / 4;
   const dim3 grid((int)(wgs < AW_GRID ? wgs : AW_GRID));
-  if (out_bf16) hipLaunchKernelGGL((adamw_unpack_kernel<unsigned short>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (unsigned short *)m, (unsigned short *)v);
+  if (out_bf16) hipLaunchKernelGGL((adamw_unpack_kernel<__bf16>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (__bf16 *)m, (__bf16 *)v);
   else hipLaunchKernelGGL((adamw_unpack_kernel<float>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (float *)m, (float *)v);
   RS_CHECK_LAUNCH("rs_adamw_unpack");
   return RS_OK;

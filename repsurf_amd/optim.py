@@ -141,6 +141,9 @@ class AdamWArgs(ctypes.Structure):           # rs_adamw_args
                 ("max_norm", ctypes.c_float), ("norm", P), ("seed", ctypes.c_uint)]
 
 
+_address, _dense = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+
+
 class _Table:
     """The host arrays of one rs_adamw_list: tensors of one type in one group."""
 
@@ -217,7 +220,7 @@ class AdamW(Adam):
             self._dev[gi] = st
             for p, a in zip(params, at):
                 self._views(st, p, a)
-        elif st["ids"] != [id(p) for p in params]:
+        elif st["ids"] != list(map(id, params)):
             raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: the parameters of a group changed after its state was made")
         return st
 
@@ -281,7 +284,8 @@ class AdamW(Adam):
             if "low" in flat:
                 rows = [(p.data_ptr(), p.data_ptr(), p.numel(), a, i) for i, (p, a) in enumerate(zip(params, st["at"]))
                         if p.dtype == torch.bfloat16 and p.numel()]
-                out["master"] = torch.zeros((st["end"],), dtype=torch.float32, device=dev)
+                all_bf16 = len(rows) == sum(p.numel() > 0 for p in params)          # (the call writes its tensors' room whole)
+                out["master"] = (torch.empty if all_bf16 else torch.zeros)((st["end"],), dtype=torch.float32, device=dev)
                 if rows:
                     _lib.call("rs_adamw_masters", _Table(rows).ref, flat["low"].data_ptr(), out["master"].data_ptr(), _lib.current_stream())
         return out
@@ -325,12 +329,17 @@ class AdamW(Adam):
             wide = None
             if self.state_bits == 8 and bits == {32}:
                 wide = {k: torch.zeros((st["end"],), dtype=torch.float32, device=dev) for k in ("exp_avg", "exp_avg_sq")}
+            to, of = [], []
             for p, a, s in zip(group["params"], st["at"], saved):
                 for name, v in s.items():
                     if wide is not None and name in wide:
-                        wide[name][a:a + p.numel()].copy_(v.reshape(-1))
+                        to.append(wide[name][a:a + p.numel()])
+                        of.append(v.reshape(-1))
                     elif name != "step" and name in self.state[p]:
-                        self.state[p][name].copy_(v)
+                        to.append(self.state[p][name])
+                        of.append(v)
+            if to:
+                torch._foreach_copy_(to, of)
             if wide is not None:
                 f = st["flat"]
                 with torch.cuda.device(dev):
@@ -343,8 +352,9 @@ class AdamW(Adam):
     def _tables(self, st, params):
         """the group's lists (fp32, bf16), rebuilt when an address changed since the last step"""
         grads = [p.grad for p in params]
-        plan = [p.data_ptr() for p in params] + [0 if g is None else g.data_ptr() for g in grads]
-        if plan == st["plan"] and all(g is None or g.is_contiguous() for g in grads) and all(p.is_contiguous() for p in params):
+        some = [g for g in grads if g is not None]
+        plan = (list(map(_address, params)), list(map(_address, some)), len(some) == len(params) or [g is None for g in grads])
+        if plan == st["plan"] and all(map(_dense, some)) and all(map(_dense, params)):
             return st["tables"], None
         rows, keep, seen = ([], []), [], set()
         for i, (p, g) in enumerate(zip(params, grads)):

@@ -2,8 +2,8 @@
 
 Tolerances.  u = 2^-24, half a step of fp32.  One update rounds m three times (difference, product in the fma's one rounding, the constant
 1 - b1) and v four times, each by at most u of the largest term; the moments contract, so over k steps |dm| <= 4 k u max|m, g|, and
-|dv| <= 5 k u max(v, g^2).  The update's ratio is then off by at most (4 + 2.5 + 6) k u relative -- the square root halves v's error; root,
-product, sum, quotient, the step size and the bias correction add six roundings -- and p by k (3 u |p| + 16 k u lr r), r the largest
+|dv| <= 5 k u max(v, g^2).  The update's ratio is then off by at most (4 + 2.5 + 9) k u relative -- the square root halves v's error; the device's
+root and reciprocal (2 u each), the sum, the product, the step size and the bias corrections add nine -- and p by k (3 u |p| + 16 k u lr r), r the largest
 ratio seen: the constant 1 - lr wd, its product with p and the sum are three roundings of at most u |p| each."""
 import copy
 
