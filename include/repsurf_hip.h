@@ -611,12 +611,13 @@ typedef struct rs_adamw_list {   /* HOST arrays of `count` entries; nothing is k
   const long long *at;           /* first element in the flat buffers */
   const int *slot;               /* step[slot] counts the tensor's updates */
 } rs_adamw_list;
+#define RS_ADAMW_DONE 528
 typedef struct rs_adamw_args {
   int bits, bf16;
   void *exp_avg, *exp_avg_sq;
   unsigned char *exp_avg_exponent, *exp_avg_sq_exponent;
   short *low;
-  int *step, *done;              /* device: updates done per tensor, advanced by the call; an int that is 0 between calls */
+  int *step, *done;              /* device: updates done per tensor, advanced by the call; RS_ADAMW_DONE ints that are 0 between calls */
   const double *hyper_dev;       /* NULL: `hyper` counts; otherwise the same seven in device memory (a captured call follows them) */
   double hyper[7];               /* lr, beta1, beta2, eps, weight_decay, ln beta1, ln beta2 */
   const double *partial;         /* NULL, or npartial sums of squares: every g is multiplied by min(1, max_norm / (norm + 1e-6)) */
@@ -628,7 +629,7 @@ typedef struct rs_adamw_args {
 int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, void *stream);
 /* Sums of squares of the list's gradients, at most RS_GRAD_SQUARE_SUMS per 80 tensors, in an order that the sizes alone fix; *used
  * (HOST) = their number, at most `room`.  l->p, at and slot are not used (p must not be NULL). */
-#define RS_GRAD_SQUARE_SUMS 512
+#define RS_GRAD_SQUARE_SUMS 1024
 int rs_grad_square_sums(const rs_adamw_list *l, int bf16, double *partial, int room, int *used, void *stream);
 /* fp32 masters of the list's bf16 parameters, flat (what lies between tensors is left as it is) */
 int rs_adamw_masters(const rs_adamw_list *l, const short *low, float *out, void *stream);

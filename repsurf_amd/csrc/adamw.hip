@@ -25,7 +25,9 @@ constexpr int AW_THREADS = 256;
 constexpr int AW_BLOCK = 256;             // elements that share an exponent
 constexpr int AW_UNROLL = 2;              // blocks a wave has in flight
 constexpr int AW_CHUNK = AW_BLOCK * (AW_THREADS / RS_WAVE) * AW_UNROLL;
+constexpr int AW_SQ_CHUNK = 8192;         // gradients a workgroup squares at a time
 constexpr int AW_MAX = 80;                // tensors per launch: the table rides in the kernel arguments
+constexpr int AW_COUNTS = RS_ADAMW_DONE / 16 - 1;      // counters of finished workgroups, below the one of all
 constexpr int AW_FIELD_M = 14, AW_FIELD_V = 30;
 
 struct AwTable {
@@ -93,6 +95,18 @@ __device__ __forceinline__ float aw_master(unsigned p_high, int low) {
 }
 // the master's word as it is kept: its upper half rounded is the parameter, its lower half, as a signed number, the remainder
 __device__ __forceinline__ unsigned aw_word(float x) { return x != x ? 0x7FC00000u : __float_as_uint(x); }
+
+// The tensor of a chunk: as many as have their running number at or below it.  All of the table's numbers are asked for at once, one per
+// lane (a bisection is seven reads, each waiting for the one before).
+struct AwFind {
+  int a, b;
+  __device__ __forceinline__ explicit AwFind(const AwTable &T) {
+    const int lane = (int)threadIdx.x & 63;
+    a = lane < T.count ? T.blk_end[lane] : 0x7FFFFFFF;
+    b = 64 + lane < T.count ? T.blk_end[64 + lane < AW_MAX ? 64 + lane : 0] : 0x7FFFFFFF;
+  }
+  __device__ __forceinline__ int operator()(int chunk) const { return (int)(__popcll(__ballot(chunk >= a)) + __popcll(__ballot(chunk >= b))); }
+};
 
 template <bool BF16> struct AwType { typedef float T; };
 template <> struct AwType<true> { typedef unsigned short T; };
@@ -263,15 +277,10 @@ adamw_kernel(AwTable T, AwArgs A) {
   const int wave = rs_uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int chunks = T.blk_end[T.count - 1];
 
-  int ti = 0, seen = -1;
+  const AwFind find(T);
+  int seen = -1;
   for (int c = (int)blockIdx.x; c < chunks; c += (int)gridDim.x) {
-    // the tensor of this chunk: the first whose running count exceeds c, by bisection above the last one (chunks only grow)
-    int lo = ti, hi = T.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (c >= T.blk_end[mid]) lo = mid + 1; else hi = mid;
-    }
-    ti = lo;
+    const int ti = find(c);
     const long long n = T.n[ti], at = T.at[ti];
     const long long b = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK + wave * (AW_BLOCK * AW_UNROLL);
     PT *__restrict__ p = (PT *)T.p[ti];
@@ -297,10 +306,18 @@ adamw_kernel(AwTable T, AwArgs A) {
     }
   }
   // The last workgroup advances the counters of this launch's tensors: every workgroup has read them by then (its reads feed its
-  // stores, in front of the barrier and the count).  No fence: nothing written here is read before the next launch.
+  // stores, in front of the barrier and the count).  No fence: nothing written here is read before the next launch.  Counted in two
+  // levels, in cache lines of their own: hundreds of workgroups that end together do not queue for one word.
   __shared__ int last;
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(A.done, 1) == (int)gridDim.x - 1;
+  if (threadIdx.x == 0) {
+    const int k = (int)blockIdx.x % AW_COUNTS, mine = ((int)gridDim.x - 1 - k) / AW_COUNTS + 1, groups = min((int)gridDim.x, AW_COUNTS);
+    last = 0;
+    if (atomicAdd(A.done + 16 * (k + 1), 1) == mine - 1) {
+      A.done[16 * (k + 1)] = 0;
+      last = atomicAdd(A.done, 1) == groups - 1;
+    }
+  }
   __syncthreads();
   if (last) {
     if ((int)threadIdx.x < T.count) A.step[T.slot[threadIdx.x]] += 1;
@@ -309,43 +326,45 @@ adamw_kernel(AwTable T, AwArgs A) {
 }
 
 // ---- the gradients' common norm -------------------------------------------------------------------------------------
-// partial[b] = sum of the squares of workgroup b's chunks.  A lane's 8 squares of a chunk are added in fp32, everything above in
-// fp64, in an order that the sizes fix.
+// partial[b] = sum of the squares of workgroup b's chunks.  A lane's 32 squares of a chunk are added in fp32, everything above in fp64, in
+// an order that the sizes fix.
 template <bool BF16>
 __global__ void __launch_bounds__(AW_THREADS)
 grad_sq_kernel(AwTable T, double *__restrict__ partial) {
   typedef typename AwType<BF16>::T PT;
+  constexpr int E = 16 / sizeof(PT), U = AW_SQ_CHUNK / (AW_THREADS * E);      // 16 bytes of a thread at a time
   __shared__ double red[AW_THREADS];
   const int chunks = T.blk_end[T.count - 1];
   double s = 0.0;
-  int ti = 0;
+  const AwFind find(T);
   for (int c = (int)blockIdx.x; c < chunks; c += (int)gridDim.x) {
-    int lo = ti, hi = T.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (c >= T.blk_end[mid]) lo = mid + 1; else hi = mid;
-    }
-    ti = lo;
-    const long long n = T.n[ti];
-    const long long base = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK;
-    const PT *__restrict__ g = (const PT *)T.g[ti];
-    constexpr int U = AW_CHUNK / (4 * AW_THREADS);
-    Four<PT> r[U];
-    if (base + AW_CHUNK <= n) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) r[u] = aw_load(g + base + (u * AW_THREADS + (int)threadIdx.x) * 4, 4);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) { const long long e = base + (u * AW_THREADS + (int)threadIdx.x) * 4; r[u] = aw_load(g + e, n - e); }
-    }
+    const int ti = find(c);
+    const long long left = T.n[ti] - (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_SQ_CHUNK;
+    const PT *__restrict__ g = (const PT *)T.g[ti] + (T.n[ti] - left);
     float a = 0.f;
+    if (left >= AW_SQ_CHUNK) {
+      unsigned w[U][4];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) __builtin_memcpy(w[u], g + (u * AW_THREADS + (int)threadIdx.x) * E, 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = aw_get(r[u], i);
+      for (int u = 0; u < U; ++u) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (BF16) {
+            const float x = __uint_as_float(w[u][i] << 16), y = __uint_as_float(w[u][i] & 0xFFFF0000u);
+            t = rs_fma(x, x, rs_fma(y, y, t));
+          } else t = rs_fma(__uint_as_float(w[u][i]), __uint_as_float(w[u][i]), t);
+        }
+        a += t;
+      }
+    } else {
+      for (int e = (int)threadIdx.x; e < (int)left; e += AW_THREADS) {
+        float x;
+        if constexpr (BF16) x = __uint_as_float((unsigned)g[e] << 16); else x = g[e];
         a = rs_fma(x, x, a);
       }
+    }
     s += (double)a;
   }
   red[threadIdx.x] = s;
@@ -410,14 +429,9 @@ adamw_unpack_kernel(long long blocks, const unsigned char *__restrict__ mc, cons
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_masters_kernel(AwTable T, const short *__restrict__ low, float *__restrict__ out) {
   const int chunks = T.blk_end[T.count - 1];
-  int ti = 0;
+  const AwFind find(T);
   for (int c = (int)blockIdx.x; c < chunks; c += (int)gridDim.x) {
-    int lo = ti, hi = T.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (c >= T.blk_end[mid]) lo = mid + 1; else hi = mid;
-    }
-    ti = lo;
+    const int ti = find(c);
     const long long n = T.n[ti], at = T.at[ti];
     const long long base = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK;
     const unsigned short *__restrict__ p = (const unsigned short *)T.p[ti];
@@ -439,7 +453,7 @@ constexpr int AW_GRID = 2048;             // 8 workgroups on each of 256 CUs
 
 // calls f(table, chunks) for runs of at most AW_MAX tensors
 template <typename F>
-int aw_tables(const rs_adamw_list *l, const char *name, F f) {
+int aw_tables(const rs_adamw_list *l, const char *name, int chunk, F f) {
   RS_REQUIRE(l && l->count >= 0 && (l->count == 0 || (l->p && l->g && l->n && l->at && l->slot)), "%s: null pointer", name);
   for (int first = 0; first < l->count; first += AW_MAX) {
     AwTable T;
@@ -450,7 +464,7 @@ int aw_tables(const rs_adamw_list *l, const char *name, F f) {
       RS_REQUIRE(l->p[k] && l->g[k] && l->n[k] > 0 && l->at[k] >= 0 && l->at[k] % AW_BLOCK == 0 && l->slot[k] >= 0,
                  "%s: tensor %d: null pointer, empty, or not at a multiple of %d elements", name, k, AW_BLOCK);
       T.p[i] = l->p[k]; T.g[i] = l->g[k]; T.n[i] = l->n[k]; T.at[i] = l->at[k]; T.slot[i] = l->slot[k];
-      chunks += (l->n[k] + AW_CHUNK - 1) / AW_CHUNK;
+      chunks += (l->n[k] + chunk - 1) / chunk;
       RS_REQUIRE(chunks < (1LL << 31), "%s: too many elements in one launch", name);
       T.blk_end[i] = (int)chunks;
     }
@@ -472,7 +486,7 @@ extern "C" int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, voi
   A.step = a->step; A.done = a->done; A.hyper_dev = a->hyper_dev;
   for (int i = 0; i < 7; ++i) A.hyper[i] = a->hyper[i];
   A.partial = a->partial; A.npartial = a->npartial; A.max_norm = a->max_norm; A.norm = a->norm; A.seed = a->seed;
-  return aw_tables(l, "rs_adamw_step", [&](const AwTable &T, int chunks) {
+  return aw_tables(l, "rs_adamw_step", AW_CHUNK, [&](const AwTable &T, int chunks) {
     const dim3 grid(chunks < AW_GRID ? chunks : AW_GRID), block(AW_THREADS);
     hipStream_t st = (hipStream_t)stream;
     if (a->bf16) {
@@ -490,7 +504,7 @@ extern "C" int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, voi
 extern "C" int rs_grad_square_sums(const rs_adamw_list *l, int bf16, double *partial, int room, int *used, void *stream) {
   RS_REQUIRE(partial && used && room >= 0, "rs_grad_square_sums: null pointer");
   *used = 0;
-  return aw_tables(l, "rs_grad_square_sums", [&](const AwTable &T, int chunks) {
+  return aw_tables(l, "rs_grad_square_sums", AW_SQ_CHUNK, [&](const AwTable &T, int chunks) {
     const int blocks = chunks < RS_GRAD_SQUARE_SUMS ? chunks : RS_GRAD_SQUARE_SUMS;
     RS_REQUIRE(*used + blocks <= room, "rs_grad_square_sums: room for %d sums, more are needed", room);
     if (bf16) hipLaunchKernelGGL((grad_sq_kernel<true>), dim3(blocks), dim3(AW_THREADS), 0, (hipStream_t)stream, T, partial + *used);
@@ -503,7 +517,7 @@ extern "C" int rs_grad_square_sums(const rs_adamw_list *l, int bf16, double *par
 
 extern "C" int rs_adamw_masters(const rs_adamw_list *l, const short *low, float *out, void *stream) {
   RS_REQUIRE(low && out, "rs_adamw_masters: null pointer");
-  return aw_tables(l, "rs_adamw_masters", [&](const AwTable &T, int chunks) {
+  return aw_tables(l, "rs_adamw_masters", AW_CHUNK, [&](const AwTable &T, int chunks) {
     hipLaunchKernelGGL(adamw_masters_kernel, dim3(chunks < AW_GRID ? chunks : AW_GRID), dim3(AW_THREADS), 0, (hipStream_t)stream, T, low, out);
     RS_CHECK_LAUNCH("rs_adamw_masters");
     return RS_OK;

@@ -128,7 +128,7 @@ class Adam(torch.optim.Optimizer):
 
 # ---------------------------------------------------------------------------------------------------------------- AdamW
 BLOCK = 256               # tensors start at multiples of it in the flat moment buffers; elements that share an 8-bit exponent
-GRAD_SQUARE_SUMS = 512    # RS_GRAD_SQUARE_SUMS
+GRAD_SQUARE_SUMS, DONE = 1024, 528      # RS_GRAD_SQUARE_SUMS, RS_ADAMW_DONE
 
 
 class AdamWList(ctypes.Structure):           # rs_adamw_list
@@ -215,7 +215,7 @@ class AdamW(Adam):
                 flat.update(exp_avg_exponent=new(end // BLOCK, torch.uint8), exp_avg_sq_exponent=new(end // BLOCK, torch.uint8))
             if any(p.dtype == torch.bfloat16 for p in params):
                 flat["low"] = new(end, torch.int16)
-            st = dict(hyper=new(7, torch.float64), host=None, step=new(len(params), torch.int32), done=new(1, torch.int32),
+            st = dict(hyper=new(7, torch.float64), host=None, step=new(len(params), torch.int32), done=new(DONE, torch.int32),
                       flat=flat, at=at, end=end, ids=[id(p) for p in params], plan=None, tables=None)
             self._dev[gi] = st
             for p, a in zip(params, at):

@@ -100,7 +100,7 @@ def test_entry_points_report_bad_arguments():
 def test_structs_match_the_header(tmp_path):
     pairs = {"rs_adamw_list": optim.AdamWList, "rs_adamw_args": optim.AdamWArgs}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "repsurf_hip.h"', 'int main(void) {',
-             'if (RS_GRAD_SQUARE_SUMS != %d) return 1;' % optim.GRAD_SQUARE_SUMS]
+             'if (RS_GRAD_SQUARE_SUMS != %d || RS_ADAMW_DONE != %d) return 1;' % (optim.GRAD_SQUARE_SUMS, optim.DONE)]
     for c, cls in pairs.items():
         lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
         lines += [f'printf("{c} {f} %zu\\n", offsetof({c}, {f}));' for f, _ in cls._fields_]

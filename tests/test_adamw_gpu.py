@@ -307,7 +307,8 @@ def test_8_bit_state_dicts(tmp_path):
 @pytest.mark.parametrize("bits,dtype", [(32, torch.float32), (8, torch.bfloat16)])
 @pytest.mark.parametrize("bound", [1.0, 1e6])
 def test_clipping_by_the_common_norm(bits, dtype, bound):
-    """The norm: fp32 squares and sums of 8 (9 roundings of u, half of them in the root), fp64 above, one rounding: 6 u."""
+    """The norm: squares and sums of at most 32 in fp32, one after the other at a tensor's end: 32 roundings of u, half of them in the root; fp64
+    above, one rounding: 17 u."""
     from repsurf_amd.optim import AdamW
     ps = make(SHAPES * 9, dtype)
     give(ps, 3)
@@ -316,7 +317,7 @@ def test_clipping_by_the_common_norm(bits, dtype, bound):
     before = [p.detach().clone() for p in ps]
     grads = [p.grad.clone() for p in ps]
     clipped.step()
-    assert abs(float(clipped.grad_norm) / want - 1) <= 6 * U
+    assert abs(float(clipped.grad_norm) / want - 1) <= 17 * U
     assert all(torch.equal(p.grad, g) for p, g in zip(ps, grads))
     m = np64(clipped.unpack_state()["exp_avg"])
     at, c = 0, min(1.0, bound / (want + 1e-6))
