@@ -155,6 +155,7 @@ class _Table:
         self.count = n
         self.list = AdamWList(n, *[ctypes.cast(a, P) for a in (self.p, self.g, self.n, self.at, self.slot)])
         self.ref = ctypes.byref(self.list)
+        self.args = self.vals = None         # the rs_adamw_args of these tensors' launches, and the hyper-parameters in it
 
 
 class AdamW(Adam):
@@ -216,7 +217,7 @@ class AdamW(Adam):
             if any(p.dtype == torch.bfloat16 for p in params):
                 flat["low"] = new(end, torch.int16)
             st = dict(hyper=new(7, torch.float64), host=None, step=new(len(params), torch.int32), done=new(DONE, torch.int32),
-                      flat=flat, at=at, end=end, ids=[id(p) for p in params], plan=None, tables=None)
+                      flat=flat, at=at, end=end, ids=[id(p) for p in params], plan=None, tables=None, key=None, vals=None)
             self._dev[gi] = st
             for p, a in zip(params, at):
                 self._views(st, p, a)
@@ -420,18 +421,27 @@ class AdamW(Adam):
                     _lib.call("rs_grad_square_sums", t.ref, bf16, partial + 8 * used, room - used, ctypes.byref(n), stream)
                     used += n.value
         for gi, group, st, tables, _ in work:
-            vals = self._hyper_values(group)
+            key = (float(group["lr"]), tuple(group["betas"]), group["eps"], group["weight_decay"])
+            if st["key"] != key:
+                st["key"], st["vals"] = key, self._hyper_values(group)
             if st["host"] is None:
                 if capturing:
                     raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: run one eager step (or sync_hyper()) before capture")
                 self.sync_hyper()
-            flat = st["flat"]
-            ptr = lambda k: flat[k].data_ptr() if k in flat else None      # noqa: E731
             for bf16, t in tables:
-                a = AdamWArgs(bits=self.state_bits, bf16=bf16, exp_avg=ptr("exp_avg"), exp_avg_sq=ptr("exp_avg_sq"),
-                              exp_avg_exponent=ptr("exp_avg_exponent"), exp_avg_sq_exponent=ptr("exp_avg_sq_exponent"), low=ptr("low"),
-                              step=st["step"].data_ptr(), done=st["done"].data_ptr(), hyper_dev=st["hyper"].data_ptr() if capturing else None,
-                              hyper=(ctypes.c_double * 7)(*vals), partial=partial if used else None, npartial=used,
-                              max_norm=self.max_grad_norm or 0.0, norm=self._norm.data_ptr() if used else None,
-                              seed=(self.seed + gi * 0x3C6EF372) & 0xFFFFFFFF)
+                a = t.args
+                if a is None:
+                    a = t.args = self._args(gi, st, bf16)
+                if t.vals is not st["vals"]:
+                    a.hyper[:], t.vals = st["vals"], st["vals"]
+                a.hyper_dev = st["hyper"].data_ptr() if capturing else None
+                a.partial, a.npartial = (partial, used) if used else (None, 0)
+                if used:
+                    a.norm, a.max_norm = self._norm.data_ptr(), self.max_grad_norm
                 _lib.call("rs_adamw_step", t.ref, ctypes.byref(a), stream)
+
+    def _args(self, gi, st, bf16):
+        ptr = lambda k: st["flat"][k].data_ptr() if k in st["flat"] else None      # noqa: E731
+        return AdamWArgs(bits=self.state_bits, bf16=bf16, exp_avg=ptr("exp_avg"), exp_avg_sq=ptr("exp_avg_sq"),
+                         exp_avg_exponent=ptr("exp_avg_exponent"), exp_avg_sq_exponent=ptr("exp_avg_sq_exponent"), low=ptr("low"),
+                         step=st["step"].data_ptr(), done=st["done"].data_ptr(), seed=(self.seed + gi * 0x3C6EF372) & 0xFFFFFFFF)
