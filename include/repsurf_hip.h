@@ -684,7 +684,7 @@ typedef struct rs_policy {
   double low, high, kl_coef;
   int *counts;                   /* scratch: RS_POLICY_COUNTS * (token_mean ? 1 : sequences) ints are enough */
   int counts_room;
-  double *partial;               /* scratch: RS_POLICY_PARTIAL doubles */
+  double *partial;               /* scratch: 3 * min(rows, RS_POLICY_GROUPS) doubles */
   int partial_room;
   float *loss, *stats, *logp;    /* logp (rows) may be NULL */
   void *dlogits;
@@ -692,7 +692,7 @@ typedef struct rs_policy {
   void *scratch;                 /* as in rs_token_logprobs */
 } rs_policy;
 #define RS_POLICY_COUNTS 64
-#define RS_POLICY_PARTIAL 6144
+#define RS_POLICY_GROUPS 8192
 int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stream);
 
 /* Measurement aid (round 6): one-thread launch that stores the device's constant-rate wall clock (s_memrealtime) in *dst when it runs;

@@ -370,6 +370,14 @@ __device__ __forceinline__ void lg_step_out(T *__restrict__ dz, int k, unsigned 
 // Long rows, one workgroup each, LDS for what its waves tell each other.  HELD (the policy loss): the row stays in registers between its
 // sum and its gradient, at most NV steps of 8 logits per thread and a tail.  Otherwise chunks of NV steps are taken in turn: their loads
 // are all in flight before the first is used, and the running maximum is corrected once per chunk.
+// logits in front of the first 16-byte border of a row whose vectors would straddle cache lines otherwise: rows of an odd number of classes.
+// The first threads take one of them each.
+template <typename T>
+__device__ __forceinline__ int lg_head(const T *z, int V) {
+  const int n = (int)((16 - ((size_t)z & 15)) & 15) / (int)sizeof(T);
+  return n < V ? n : V;
+}
+
 // (WAVES per SIMD bound the registers: left alone, the compiler interleaves the steps until two waves are all that fits)
 template <typename T, int MODE, int THREADS, int NV, bool HELD, int WAVES>
 __global__ void __launch_bounds__(THREADS, WAVES)
@@ -378,28 +386,32 @@ long_kernel(Rows R, Policy P, Outs O) {
   __shared__ float red_m[2][W];
   __shared__ double red_s[2][W];
   __shared__ float red_c[2];
-  const int tid = (int)threadIdx.x, wave = tid >> 6, V = R.classes;
+  const int tid = (int)threadIdx.x, wave = tid >> 6;
   const unsigned off = (unsigned)tid * (LG_VEC * sizeof(T));
-  const int full = V / STEP, last = full * STEP + tid * LG_VEC;          // whole steps, and the thread's first logit behind them
   double add[3] = {0.0, 0.0, 0.0};
   int turn = 0;                       // scratch of two rows in turn: a row's last reader is a barrier ahead of the next but one's writer
   for (long long row = blockIdx.x; row < R.rows; row += gridDim.x) {
     const Row w = lg_row(R, row);
     const T *__restrict__ z = (const T *)R.z + row * R.ld;
-    T *__restrict__ dz = O.dz ? (T *)O.dz + row * V : nullptr;
+    T *__restrict__ dz = O.dz ? (T *)O.dz + row * R.classes : nullptr;
     if (!w.counts || w.bad) {
       const float fill = lg_void(R, P, O, w, tid == 0, MODE == LG_POLICY, add);
       if (MODE == LG_POLICY && dz)
-        for (int j = tid * LG_VEC; j < V; j += STEP) lg_fill(dz + j, V - j, fill);
+        for (int j = tid * LG_VEC; j < R.classes; j += STEP) lg_fill(dz + j, R.classes - j, fill);
       continue;
     }
     turn ^= 1;
     Vec<T> v[NV], tail;
-    float m = -INFINITY, M;
+    float M;
     double s = 0.0;
     Pre pre{1.0, 0.f, 0.f, 0.f};
     const float zy = (float)z[w.y];
+    const int head = lg_head(z, R.classes), V = R.classes - head;          // from here on, V logits from z + head
+    const float first = tid < head ? (float)z[tid] : -INFINITY;
+    z += head;
+    const int full = V / STEP, last = full * STEP + tid * LG_VEC;          // whole steps, and the thread's first logit behind them
     if (MODE == LG_POLICY && wave == 0) pre = lg_pre(R, P, w);
+    float m = HELD ? first : -INFINITY;
     if (HELD) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) lg_step<T, THREADS>(z, k, off, k < full, v[k]);
@@ -423,13 +435,13 @@ long_kernel(Rows R, Policy P, Outs O) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) lg_step<T, THREADS>(z, k0 + k, off, k0 + k < full, v[k]);
       tail = lg_load(z + last, V - last);
-      float top = lg_top(tail, m);
+      float top = lg_top(tail, fmaxf(m, first));
 #pragma unroll
       for (int k = 0; k < NV; ++k) if (k0 + k < full) top = lg_top(v[k], top);
       if (top > m) { s *= (double)lg_exp(m - top); m = top; }
 #pragma unroll
       for (int k = 0; k < NV; ++k) if (k0 + k < full) s += lg_sum(v[k], lg_base(m));
-      s += lg_sum(tail, lg_base(m));
+      s += lg_sum(tail, lg_base(m)) + (double)lg_exp(first - lg_base(m));
     }
     M = lg_lanes_max<64>(m);
     if ((tid & 63) == 0) red_m[turn][wave] = M;
@@ -441,7 +453,7 @@ long_kernel(Rows R, Policy P, Outs O) {
     if (HELD) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) if (k < full) { s += lg_sum(v[k], base); lg_forget(v[k]); }
-      s += lg_sum(tail, base);
+      s += lg_sum(tail, base) + (double)lg_exp(first - base);
       lg_forget(tail);
     } else if (m != -INFINITY) s *= (double)lg_exp(m - base);
     s = lg_lanes_sum<64>(s);
@@ -459,11 +471,13 @@ long_kernel(Rows R, Policy P, Outs O) {
       __syncthreads();
       c = red_c[turn];
       const float scale = -c * (1.f / (float)s);
-      const int y = (int)w.y;
+      const int y = (int)w.y - head;
       if (c != c) {
-        for (int j = tid * LG_VEC; j < V; j += STEP) lg_fill(dz + j, V - j, c);
+        for (int j = tid * LG_VEC; j < R.classes; j += STEP) lg_fill(dz + j, R.classes - j, c);
         continue;
       }
+      if (tid < head) dz[tid] = (T)(lg_exp(first - base) * scale + (tid == (int)w.y ? c : 0.f));
+      dz += head;
       if (HELD) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) if (k < full) lg_step_out<T, THREADS>(dz, k, off, tid, v[k], base, scale, c, y);
@@ -496,28 +510,31 @@ long_back_kernel(Rows R, Outs O, int parts) {
   if (O.skip_unit && up == 1.f) return;
   const int tid = (int)threadIdx.x, V = R.classes;
   const unsigned off = (unsigned)tid * (LG_VEC * sizeof(T));
-  for (long long row = blockIdx.y; row < R.rows; row += gridDim.y)
-  for (int part = blockIdx.x; part < parts; part += gridDim.x) {
-    const int j0 = part * (STEP * NV);
+  for (long long row = blockIdx.y; row < R.rows; row += gridDim.y) {
     const Row w = lg_row(R, row);
-    const T *__restrict__ z = (const T *)R.z + row * R.ld + j0;
-    T *__restrict__ dz = (T *)O.dz + row * V + j0;
-    const int left = V - j0, full = left / STEP < NV ? left / STEP : NV, y = (int)w.y - j0;
     float c = 0.f;
     if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w.owner : row] * up;
+    const T *__restrict__ z = (const T *)R.z + row * R.ld;
+    T *__restrict__ dz = (T *)O.dz + row * V;
     if (c == 0.f || c != c) {
-      for (int j = tid * LG_VEC; j < left && j < STEP * NV; j += STEP) lg_fill(dz + j, left - j, c);
+      for (int j = ((int)blockIdx.x * 256 + tid) * LG_VEC; j < V; j += (int)gridDim.x * STEP) lg_fill(dz + j, V - j, c);
       continue;
     }
-    Vec<T> v[NV];
+    const int head = lg_head(z, V);
+    for (int part = blockIdx.x; part < parts; part += gridDim.x) {
+      const int j0 = head + part * (STEP * NV), left = V - j0, y = (int)w.y - j0;
+      const int full = left <= 0 ? 0 : (left / STEP < NV ? left / STEP : NV);
+      Vec<T> v[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) lg_step<T, 256>(z, k, off, k < full, v[k]);
-    const float2 st = O.stat[row];
-    const float base = lg_base(st.x), scale = -c * st.y;
+      for (int k = 0; k < NV; ++k) lg_step<T, 256>(z + j0, k, off, k < full, v[k]);
+      const float2 st = O.stat[row];
+      const float base = lg_base(st.x), scale = -c * st.y;
+      if (part == 0 && tid < head) dz[tid] = (T)(lg_exp((float)z[tid] - base) * scale + (tid == (int)w.y ? c : 0.f));
 #pragma unroll
-    for (int k = 0; k < NV; ++k) if (k < full) lg_step_out<T, 256>(dz, k, off, tid, v[k], base, scale, c, y);
-    const int last = full * STEP + tid * LG_VEC;
-    if (full < NV && last < left) lg_gradient(dz + last, left - last, lg_load(z + last, left - last), base, scale, c, last, y);
+      for (int k = 0; k < NV; ++k) if (k < full) lg_step_out<T, 256>(dz + j0, k, off, tid, v[k], base, scale, c, y);
+      const int last = full * STEP + tid * LG_VEC;
+      if (full < NV && last < left) lg_gradient(dz + j0 + last, left - last, lg_load(z + j0 + last, left - last), base, scale, c, last, y);
+    }
   }
 }
 
@@ -601,20 +618,25 @@ count_kernel(long long rows, const int *__restrict__ offset, const long long *__
   if (threadIdx.x == 0) counts[(long long)q * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
+template <int WAVES>
 __device__ __forceinline__ double lg_block_sum(double x, double *red) {
   x = lg_lanes_sum<64>(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  x = red[0];
+#pragma unroll
+  for (int k = 1; k < WAVES; ++k) x += red[k];
+  return x;
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 policy_sum_kernel(int n, const double *__restrict__ partial, float *__restrict__ loss, float *__restrict__ stats) {
-  __shared__ double red[4];
+  __shared__ double red[16];
   double a = 0.0, b = 0.0, c = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) { a += partial[3 * i]; b += partial[3 * i + 1]; c += partial[3 * i + 2]; }
-  a = lg_block_sum(a, red); b = lg_block_sum(b, red); c = lg_block_sum(c, red);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 1024) { a += partial[3 * i]; b += partial[3 * i + 1]; c += partial[3 * i + 2]; }
+  a = lg_block_sum<16>(a, red); b = lg_block_sum<16>(b, red); c = lg_block_sum<16>(c, red);
   if (threadIdx.x == 0) { *loss = (float)a; stats[0] = (float)b; stats[1] = (float)c; }
 }
 
@@ -628,8 +650,8 @@ sequence_kernel(Rows R, const double *__restrict__ logp, int average, double *__
   if (b > R.rows) b = R.rows;
   double s = 0.0, n = 0.0;
   for (long long i = a + threadIdx.x; i < b; i += 256) { s += logp[i]; n += R.target[i] != R.ignore ? 1.0 : 0.0; }
-  s = lg_block_sum(s, red);
-  n = lg_block_sum(n, red);
+  s = lg_block_sum<4>(s, red);
+  n = lg_block_sum<4>(n, red);
   if (threadIdx.x == 0) {
     const double k = average ? 1.0 / fmax(n, 1.0) : 1.0;
     if (sums) sums[q] = s * k;
@@ -654,7 +676,7 @@ pairs_kernel(int pairs, const double *__restrict__ sums, const float *__restrict
     coef[i] = (float)(slope * each[i]);
     coef[pairs + i] = (float)(-slope * each[pairs + i]);
   }
-  t = lg_block_sum(t, red);
+  t = lg_block_sum<4>(t, red);
   if (threadIdx.x == 0) *loss = (float)(t / pairs);
 }
 
@@ -669,7 +691,10 @@ Rows rows_of(const rs_logits *l) {
   return Rows{l->logits, l->rows, l->ld, l->classes, l->sequences, l->target, l->ignore_index, l->offset, l->bad_labels};
 }
 
-constexpr int LG_GRID = 2048;             // 8 workgroups of 256 threads on each of 256 CUs
+constexpr int LG_GRID = 2048;             // 8 workgroups of 256 threads on each of 256 CUs, for rows that are much alike
+// Long rows get a workgroup each: some cost nothing (prompts), and 6208 rows dealt to 2048 workgroups beforehand leave a third of the chip idle
+// at the end.  The policy loss's stop where its partial sums would cost more.
+constexpr int LG_LONG_GRID = 1 << 20;
 constexpr int LG_SHORT = 4096;            // classes of the longest row that a wave holds
 constexpr int LG_FEW = 256, LG_PARTS = 64;
 static_assert(LG_PARTS == RS_LOGITS_PARTS && LG_FEW == RS_LOGITS_FEW_ROWS, "room of the callers' scratch");
@@ -700,10 +725,11 @@ int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &
   if constexpr (MODE == LG_BACK) {
     constexpr int NV = 4;
     const int parts = (V + 256 * LG_VEC * NV - 1) / (256 * LG_VEC * NV), across = lesser(parts, LG_GRID);
-    hipLaunchKernelGGL((long_back_kernel<T, NV>), dim3(across, lesser(R.rows, 2 * LG_GRID / across)), dim3(256), 0, st, R, O, parts);
+    // (a launch that most often finds nothing to do is kept small: 63 000 workgroups that leave at once take 26 us)
+    hipLaunchKernelGGL((long_back_kernel<T, NV>), dim3(across, lesser(R.rows, O.skip_unit ? 2 * LG_GRID / across : 65535)), dim3(256), 0, st, R, O, parts);
     return 0;
   } else {
-#define LG_RUN_LONG(TH, N, H, WV) { const int g = lesser(R.rows, LG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H, WV>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
+#define LG_RUN_LONG(TH, N, H, WV) { const int g = lesser(R.rows, MODE == LG_POLICY ? RS_POLICY_GROUPS : LG_LONG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H, WV>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
     if constexpr (MODE == LG_POLICY) {       // (without a gradient too: the loss has the same bits either way)
       constexpr int K = sizeof(T) / 2;       // 8 logits: 4 or 8 registers of a thread
       if (V < 10240) LG_RUN_LONG(256, 4, true, K == 1 ? 5 : 4)
@@ -811,8 +837,9 @@ extern "C" int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stre
   splits = splits < 1 ? 1 : (splits > 64 ? 64 : splits);
   RS_REQUIRE((long long)parts * splits <= p->counts_room, "rs_policy_loss: room for %d counts, %lld are needed", p->counts_room, parts * splits);
   RS_REQUIRE(parts <= 65535, "rs_policy_loss: %d sequences (at most 65535)", parts);
-  RS_REQUIRE(p->partial_room >= RS_POLICY_PARTIAL, "rs_policy_loss: room for %d partial sums, %d are needed", p->partial_room, RS_POLICY_PARTIAL);
-  static_assert(RS_POLICY_PARTIAL >= 3 * LG_GRID, "room of the callers' partial sums");
+  RS_REQUIRE(p->partial_room >= 3 * lesser(l->rows, RS_POLICY_GROUPS), "rs_policy_loss: room for %d partial sums, %d are needed", p->partial_room,
+             3 * lesser(l->rows, RS_POLICY_GROUPS));
+  static_assert(RS_POLICY_GROUPS >= LG_GRID && RS_POLICY_GROUPS >= LG_FEW, "every workgroup leaves partial sums");
   // (all rows of a token mean: those of the offsets' last sequence end them)
   hipLaunchKernelGGL(count_kernel, dim3((int)splits, parts), dim3(256), 0, st, l->rows,
                      l->offset ? (p->token_mean ? l->offset + l->sequences - 1 : l->offset) : nullptr, l->target, l->ignore_index, p->counts);
@@ -822,7 +849,7 @@ extern "C" int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stre
                    p->coef, p->partial};
     n = run_rows<LG_POLICY>(l, P, Outs{p->logp, nullptr, (float2 *)p->stat, p->dlogits, nullptr, nullptr, 0}, p->scratch, st);
   }
-  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(256), 0, st, n, p->partial, p->loss, p->stats);
+  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, n, p->partial, p->loss, p->stats);
   RS_CHECK_LAUNCH("rs_policy_loss");
   return RS_OK;
 }

@@ -24,7 +24,7 @@ from . import _lib, head
 
 P, c_int, c_ll, c_double = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-POLICY_COUNTS, POLICY_PARTIAL = 64, 6144          # RS_POLICY_COUNTS, RS_POLICY_PARTIAL
+POLICY_COUNTS, POLICY_GROUPS = 64, 8192          # RS_POLICY_COUNTS, RS_POLICY_GROUPS
 FEW_ROWS, PARTS = 256, 64                         # RS_LOGITS_FEW_ROWS, RS_LOGITS_PARTS
 
 PolicyLoss = namedtuple("PolicyLoss", "loss logp kl clip_fraction")
@@ -240,11 +240,12 @@ class _Policy(Function):
     def forward(ctx, logits, target, old, adv, ref, offset, low, high, kl_coef, token_mean, ignore_index, grad):
         rows = logits.shape[0]
         loss, stats, logp = _new(logits), _new(logits, 2), _new(logits, rows)
+        partial = 3 * min(rows, POLICY_GROUPS)
         room, counts = _scratch_floats(logits), POLICY_COUNTS * (1 if token_mean else offset.numel())
         # one buffer: partial sums (fp64), scratch, counts, then the rows' stat (pairs: at an even place) and coef
-        work = _new(logits, 2 * POLICY_PARTIAL + room + counts + (3 * rows if grad else 0))
+        work = _new(logits, 2 * partial + room + counts + (3 * rows if grad else 0))
         at = work.data_ptr()
-        scratch = at + 8 * POLICY_PARTIAL
+        scratch = at + 8 * partial
         count_at = scratch + 4 * room
         stat = count_at + 4 * counts
         coef = stat + 8 * rows
@@ -252,7 +253,7 @@ class _Policy(Function):
         held = grad and rows > 0
         desc = _desc(logits, target, ignore_index, offset)
         p = PolicyDesc(old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr(), int(adv.dim() == 2), int(token_mean), low, high, kl_coef,
-                       count_at, counts, at, POLICY_PARTIAL, loss.data_ptr(), stats.data_ptr(), logp.data_ptr(), d.data_ptr() if held else None,
+                       count_at, counts, at, partial, loss.data_ptr(), stats.data_ptr(), logp.data_ptr(), d.data_ptr() if held else None,
                        coef if held else None, stat if held else None, scratch if room else None)
         _call(logits.device, "rs_policy_loss", ctypes.byref(desc), ctypes.byref(p))
         if grad:

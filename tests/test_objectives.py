@@ -59,7 +59,7 @@ def test_entry_points_report_bad_arguments():
         return ctypes.byref(O.PolicyDesc(**d))
 
     for bad in (dict(loss=None), dict(stats=None), dict(partial=None), dict(counts=None), dict(old_logp=None), dict(advantages=None), dict(dlogits=256),
-                dict(coef=256), dict(token_mean=0), dict(advantages_per_sequence=1), dict(counts_room=0), dict(partial_room=6143)):
+                dict(coef=256), dict(token_mean=0), dict(advantages_per_sequence=1), dict(counts_room=0), dict(partial_room=11)):
         with pytest.raises(_lib.RepSurfHipError, match="rs_policy_loss"):
             _lib.call("rs_policy_loss", rows(), policy(**bad), None)
     _lib.call("rs_token_logprobs", rows(rows=0), 256, None, None, None, None)          # nothing to do
@@ -69,7 +69,7 @@ def test_entry_points_report_bad_arguments():
 def test_structs_match_the_header(tmp_path):
     pairs = {"rs_logits": O.LogitsDesc, "rs_policy": O.PolicyDesc}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "repsurf_hip.h"', 'int main(void) {',
-             f'if (RS_POLICY_COUNTS != {O.POLICY_COUNTS} || RS_POLICY_PARTIAL != {O.POLICY_PARTIAL} || RS_LOGITS_FEW_ROWS != {O.FEW_ROWS} || RS_LOGITS_PARTS != {O.PARTS}) return 1;']
+             f'if (RS_POLICY_COUNTS != {O.POLICY_COUNTS} || RS_POLICY_GROUPS != {O.POLICY_GROUPS} || RS_LOGITS_FEW_ROWS != {O.FEW_ROWS} || RS_LOGITS_PARTS != {O.PARTS}) return 1;']
     for c, cls in pairs.items():
         lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
         lines += [f'printf("{c} {f} %zu\\n", offsetof({c}, {f}));' for f, _ in cls._fields_]
