@@ -620,10 +620,7 @@ typedef struct rs_adamw_args {
   int *step, *done;              /* device: updates done per tensor, advanced by the call; RS_ADAMW_DONE ints that are 0 between calls */
   const double *hyper_dev;       /* NULL: `hyper` counts; otherwise the same seven in device memory (a captured call follows them) */
   double hyper[7];               /* lr, beta1, beta2, eps, weight_decay, ln beta1, ln beta2 */
-  const double *partial;         /* NULL, or npartial sums of squares: every g is multiplied by min(1, max_norm / (norm + 1e-6)) */
-  int npartial;
-  float max_norm;
-  float *norm;                   /* device: receives the norm */
+  const float *clip;             /* device: a factor for every gradient (rs_grad_norm's out + 1); NULL: 1 */
   unsigned seed;
 } rs_adamw_args;
 int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, void *stream);
@@ -631,6 +628,8 @@ int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, void *stream);
  * (HOST) = their number, at most `room`.  l->p, at and slot are not used (p must not be NULL). */
 #define RS_GRAD_SQUARE_SUMS 1024
 int rs_grad_square_sums(const rs_adamw_list *l, int bf16, double *partial, int room, int *used, void *stream);
+/* out (2, device) = the root of the n sums' sum, and min(1, max_norm / (that + 1e-6)) */
+int rs_grad_norm(int n, const double *partial, float max_norm, float *out, void *stream);
 /* fp32 masters of the list's bf16 parameters, flat (what lies between tensors is left as it is) */
 int rs_adamw_masters(const rs_adamw_list *l, const short *low, float *out, void *stream);
 /* flat fp32 moments (n a multiple of 256) -> 8 bits, to nearest; 8 bits -> values in fp32 or bf16 (which holds them exactly, down to

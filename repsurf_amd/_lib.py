@@ -92,6 +92,7 @@ SIGNATURES = {
     "rs_timestamp": [P, P],
     "rs_adamw_step": [P, P, P],
     "rs_grad_square_sums": [P, c_int, P, c_int, P, P],
+    "rs_grad_norm": [c_int, P, ctypes.c_float, P, P],
     "rs_adamw_masters": [P, P, P, P],
     "rs_adamw_pack": [c_ll, P, P, P, P, P, P, P],
     "rs_adamw_unpack": [c_ll, P, P, P, P, c_int, P, P, P],

@@ -47,10 +47,7 @@ struct AwArgs {
   int *step, *done;
   const double *hyper_dev;                // captured launches read their hyper-parameters from device memory
   double hyper[7];                        // lr, beta1, beta2, eps, weight_decay, ln beta1, ln beta2
-  const double *partial;                  // sums of squares of the gradients, or null
-  int npartial;
-  float max_norm;
-  float *norm;
+  const float *clip;                      // a factor for every gradient, or null
   unsigned seed;
 };
 
@@ -153,22 +150,6 @@ __device__ __forceinline__ unsigned aw_wave_pair_max(unsigned v) {
   return rs_uniform((int)aw_pair_max((unsigned)s[0], (unsigned)s[1]));
 }
 
-// max(1, ...) of torch.nn.utils.clip_grad_norm_: max_norm / (norm + 1e-6), at most 1; a norm that is not a number stays one
-__device__ __forceinline__ float aw_clip(const double *partial, int n, float max_norm, float *norm_out, double *red) {
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += AW_THREADS) s += partial[i];
-  red[threadIdx.x] = s;
-  __syncthreads();
-  for (int off = AW_THREADS / 2; off > 0; off >>= 1) {
-    if ((int)threadIdx.x < off) red[threadIdx.x] += red[threadIdx.x + off];
-    __syncthreads();
-  }
-  const float norm = (float)sqrt(red[0]);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-  const float c = max_norm / (norm + 1e-6f);
-  return c > 1.f ? 1.f : c;
-}
-
 // what a launch's elements share, and what a tensor's do
 struct AwShared {
   float eps, decay, omb1, b2, omb2, clip;
@@ -266,43 +247,34 @@ template <bool BF16, int BITS>
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_kernel(AwTable T, AwArgs A) {
   typedef typename AwType<BF16>::T PT;
-  __shared__ double red[AW_THREADS];
   double lr = A.hyper[0], beta1 = A.hyper[1], beta2 = A.hyper[2], eps64 = A.hyper[3], wd = A.hyper[4], lnb1 = A.hyper[5], lnb2 = A.hyper[6];
   if (A.hyper_dev) {
     lr = A.hyper_dev[0]; beta1 = A.hyper_dev[1]; beta2 = A.hyper_dev[2]; eps64 = A.hyper_dev[3]; wd = A.hyper_dev[4];
     lnb1 = A.hyper_dev[5]; lnb2 = A.hyper_dev[6];
   }
   AwShared S{(float)eps64, (float)(1.0 - lr * wd), (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), 1.f, 0.f, 1.f, 0u};
-  if (A.partial) S.clip = aw_clip(A.partial, A.npartial, A.max_norm, A.norm, red);
+  if (A.clip) S.clip = *A.clip;
   const int wave = rs_uniform((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-  const int chunks = T.blk_end[T.count - 1];
 
-  const AwFind find(T);
-  int seen = -1;
-  for (int c = (int)blockIdx.x; c < chunks; c += (int)gridDim.x) {
-    const int ti = find(c);
-    const long long n = T.n[ti], at = T.at[ti];
-    const long long b = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK + wave * (AW_BLOCK * AW_UNROLL);
-    PT *__restrict__ p = (PT *)T.p[ti];
-    const PT *__restrict__ g = (const PT *)T.g[ti];
-    const bool whole = b + AW_BLOCK * AW_UNROLL <= n;
-    AwBlocks<BF16, BITS, AW_UNROLL, true> W;
-    if (whole) W.load(A, p, g, at, b, lane, n);               // (in front of the step count, which the loads do not need)
-    if (ti != seen) {
-      seen = ti;
-      const int t = A.step[T.slot[ti]] + 1;
-      // 1 - beta^t as -expm1(t ln beta): fp32 loses nothing where beta^t is near 1
-      S.step_size = (float)(lr / (double)-expm1f((float)(lnb1 * t)));
-      S.inv_bc2 = 1.f / sqrtf(-expm1f((float)(lnb2 * t)));
-      S.key = aw_mix(A.seed + (unsigned)t * AW_PHI);
-    }
-    if (whole) W.update(A, S, p, at, b, lane, n);
-    else {
-      for (int u = 0; u < AW_UNROLL && b + u * AW_BLOCK < n; ++u) {
-        AwBlocks<BF16, BITS, 1, false> E;
-        E.load(A, p, g, at, b + u * AW_BLOCK, lane, n);
-        E.update(A, S, p, at, b + u * AW_BLOCK, lane, n);
-      }
+  const int c = (int)blockIdx.x, ti = AwFind(T)(c);
+  const long long n = T.n[ti], at = T.at[ti];
+  const long long b = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK + wave * (AW_BLOCK * AW_UNROLL);
+  PT *__restrict__ p = (PT *)T.p[ti];
+  const PT *__restrict__ g = (const PT *)T.g[ti];
+  const bool whole = b + AW_BLOCK * AW_UNROLL <= n;
+  AwBlocks<BF16, BITS, AW_UNROLL, true> W;
+  if (whole) W.load(A, p, g, at, b, lane, n);                 // (in front of the step count, which the loads do not need)
+  const int t = A.step[T.slot[ti]] + 1;
+  // 1 - beta^t as -expm1(t ln beta): fp32 loses nothing where beta^t is near 1
+  S.step_size = (float)(lr / (double)-expm1f((float)(lnb1 * t)));
+  S.inv_bc2 = 1.f / sqrtf(-expm1f((float)(lnb2 * t)));
+  S.key = aw_mix(A.seed + (unsigned)t * AW_PHI);
+  if (whole) W.update(A, S, p, at, b, lane, n);
+  else {
+    for (int u = 0; u < AW_UNROLL && b + u * AW_BLOCK < n; ++u) {
+      AwBlocks<BF16, BITS, 1, false> E;
+      E.load(A, p, g, at, b + u * AW_BLOCK, lane, n);
+      E.update(A, S, p, at, b + u * AW_BLOCK, lane, n);
     }
   }
   // The last workgroup advances the counters of this launch's tensors: every workgroup has read them by then (its reads feed its
@@ -376,6 +348,26 @@ grad_sq_kernel(AwTable T, double *__restrict__ partial) {
   if (threadIdx.x == 0) partial[blockIdx.x] = red[0];
 }
 
+// the norm of all, and the factor of torch.nn.utils.clip_grad_norm_: max_norm / (norm + 1e-6), at most 1; a norm that is no number stays none
+__global__ void __launch_bounds__(AW_THREADS)
+grad_norm_kernel(int n, const double *__restrict__ partial, float max_norm, float *__restrict__ out) {
+  __shared__ double red[AW_THREADS];
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += AW_THREADS) s += partial[i];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int off = AW_THREADS / 2; off > 0; off >>= 1) {
+    if ((int)threadIdx.x < off) red[threadIdx.x] += red[threadIdx.x + off];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const float norm = (float)sqrt(red[0]), c = max_norm / (norm + 1e-6f);
+    out[0] = norm;
+    out[1] = c > 1.f ? 1.f : c;
+  }
+}
+
 // ---- 8-bit moments <-> values, flat ---------------------------------------------------------------------------------
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_pack_kernel(long long blocks, const float *__restrict__ m, const float *__restrict__ v, unsigned char *__restrict__ mc,
@@ -428,28 +420,22 @@ adamw_unpack_kernel(long long blocks, const unsigned char *__restrict__ mc, cons
 // masters of bf16 parameters into a flat fp32 buffer, zeros up to the next tensor
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_masters_kernel(AwTable T, const short *__restrict__ low, float *__restrict__ out) {
-  const int chunks = T.blk_end[T.count - 1];
-  const AwFind find(T);
-  for (int c = (int)blockIdx.x; c < chunks; c += (int)gridDim.x) {
-    const int ti = find(c);
-    const long long n = T.n[ti], at = T.at[ti];
-    const long long base = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK;
-    const unsigned short *__restrict__ p = (const unsigned short *)T.p[ti];
+  const int c = (int)blockIdx.x, ti = AwFind(T)(c);
+  const long long n = T.n[ti], at = T.at[ti];
+  const long long base = (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_CHUNK;
+  const unsigned short *__restrict__ p = (const unsigned short *)T.p[ti];
 #pragma unroll
-    for (int u = 0; u < AW_CHUNK / (4 * AW_THREADS); ++u) {
-      const long long e = base + (u * AW_THREADS + (int)threadIdx.x) * 4, left = n - e;
-      if (e >= (n + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK) continue;
-      const Four<unsigned short> r = aw_load(p + e, left);
-      const Four<short> l = aw_load(low + at + e, 4);
-      Four<float> x;
+  for (int u = 0; u < AW_CHUNK / (4 * AW_THREADS); ++u) {
+    const long long e = base + (u * AW_THREADS + (int)threadIdx.x) * 4, left = n - e;
+    if (e >= (n + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK) continue;
+    const Four<unsigned short> r = aw_load(p + e, left);
+    const Four<short> l = aw_load(low + at + e, 4);
+    Four<float> x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x.w[i] = i < left ? __float_as_uint(aw_master(aw_high(r, i), aw_get(l, i))) : 0u;
-      aw_store(out + at + e, x, 4);
-    }
+    for (int i = 0; i < 4; ++i) x.w[i] = i < left ? __float_as_uint(aw_master(aw_high(r, i), aw_get(l, i))) : 0u;
+    aw_store(out + at + e, x, 4);
   }
 }
-
-constexpr int AW_GRID = 2048;             // 8 workgroups on each of 256 CUs
 
 // calls f(table, chunks) for runs of at most AW_MAX tensors
 template <typename F>
@@ -480,14 +466,13 @@ extern "C" int rs_adamw_step(const rs_adamw_list *l, const rs_adamw_args *a, voi
   RS_REQUIRE(a && a->exp_avg && a->exp_avg_sq && a->step && a->done, "rs_adamw_step: null pointer");
   RS_REQUIRE(a->bits == 32 || (a->bits == 8 && a->exp_avg_exponent && a->exp_avg_sq_exponent), "rs_adamw_step: bits=%d (32, or 8 with exponents)", a->bits);
   RS_REQUIRE(!a->bf16 || a->low, "rs_adamw_step: bf16 parameters need the masters' low halves");
-  RS_REQUIRE(!a->partial || (a->npartial > 0 && a->norm && a->max_norm > 0.f), "rs_adamw_step: partial sums without their number, a norm or a bound");
   AwArgs A;
   A.m = a->exp_avg; A.v = a->exp_avg_sq; A.me = a->exp_avg_exponent; A.ve = a->exp_avg_sq_exponent; A.low = a->low;
   A.step = a->step; A.done = a->done; A.hyper_dev = a->hyper_dev;
   for (int i = 0; i < 7; ++i) A.hyper[i] = a->hyper[i];
-  A.partial = a->partial; A.npartial = a->npartial; A.max_norm = a->max_norm; A.norm = a->norm; A.seed = a->seed;
+  A.clip = a->clip; A.seed = a->seed;
   return aw_tables(l, "rs_adamw_step", AW_CHUNK, [&](const AwTable &T, int chunks) {
-    const dim3 grid(chunks < AW_GRID ? chunks : AW_GRID), block(AW_THREADS);
+    const dim3 grid(chunks), block(AW_THREADS);
     hipStream_t st = (hipStream_t)stream;
     if (a->bf16) {
       if (a->bits == 8) hipLaunchKernelGGL((adamw_kernel<true, 8>), grid, block, 0, st, T, A);
@@ -515,10 +500,18 @@ extern "C" int rs_grad_square_sums(const rs_adamw_list *l, int bf16, double *par
   });
 }
 
+extern "C" int rs_grad_norm(int n, const double *partial, float max_norm, float *out, void *stream) {
+  RS_REQUIRE(n > 0 && partial && out, "rs_grad_norm: null pointer or no sums");
+  RS_REQUIRE(max_norm > 0.f, "rs_grad_norm: max_norm=%g", max_norm);
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(AW_THREADS), 0, (hipStream_t)stream, n, partial, max_norm, out);
+  RS_CHECK_LAUNCH("rs_grad_norm");
+  return RS_OK;
+}
+
 extern "C" int rs_adamw_masters(const rs_adamw_list *l, const short *low, float *out, void *stream) {
   RS_REQUIRE(low && out, "rs_adamw_masters: null pointer");
   return aw_tables(l, "rs_adamw_masters", AW_CHUNK, [&](const AwTable &T, int chunks) {
-    hipLaunchKernelGGL(adamw_masters_kernel, dim3(chunks < AW_GRID ? chunks : AW_GRID), dim3(AW_THREADS), 0, (hipStream_t)stream, T, low, out);
+    hipLaunchKernelGGL(adamw_masters_kernel, dim3(chunks), dim3(AW_THREADS), 0, (hipStream_t)stream, T, low, out);
     RS_CHECK_LAUNCH("rs_adamw_masters");
     return RS_OK;
   });
@@ -530,7 +523,7 @@ extern "C" int rs_adamw_pack(long long n, const float *m, const float *v, unsign
   if (n == 0) return RS_OK;
   RS_REQUIRE(m && v && mc && vc && me && ve, "rs_adamw_pack: null pointer");
   const long long blocks = n / AW_BLOCK, wgs = (blocks + 3) / 4;
-  hipLaunchKernelGGL(adamw_pack_kernel, dim3((int)(wgs < AW_GRID ? wgs : AW_GRID)), dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, m, v, mc, vc, me, ve);
+  hipLaunchKernelGGL(adamw_pack_kernel, dim3((int)(wgs < (1 << 30) ? wgs : (1 << 30))), dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, m, v, mc, vc, me, ve);
   RS_CHECK_LAUNCH("rs_adamw_pack");
   return RS_OK;
 }
@@ -541,7 +534,7 @@ extern "C" int rs_adamw_unpack(long long n, const unsigned char *mc, const unsig
   if (n == 0) return RS_OK;
   RS_REQUIRE(m && v && mc && vc && me && ve, "rs_adamw_unpack: null pointer");
   const long long blocks = n / AW_BLOCK, wgs = (blocks + 3) / 4;
-  const dim3 grid((int)(wgs < AW_GRID ? wgs : AW_GRID));
+  const dim3 grid((int)(wgs < (1 << 30) ? wgs : (1 << 30)));
   if (out_bf16) hipLaunchKernelGGL((adamw_unpack_kernel<__bf16>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (__bf16 *)m, (__bf16 *)v);
   else hipLaunchKernelGGL((adamw_unpack_kernel<float>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (float *)m, (float *)v);
   RS_CHECK_LAUNCH("rs_adamw_unpack");

@@ -137,8 +137,7 @@ class AdamWList(ctypes.Structure):           # rs_adamw_list
 
 class AdamWArgs(ctypes.Structure):           # rs_adamw_args
     _fields_ = [("bits", c_int), ("bf16", c_int), ("exp_avg", P), ("exp_avg_sq", P), ("exp_avg_exponent", P), ("exp_avg_sq_exponent", P),
-                ("low", P), ("step", P), ("done", P), ("hyper_dev", P), ("hyper", ctypes.c_double * 7), ("partial", P), ("npartial", c_int),
-                ("max_norm", ctypes.c_float), ("norm", P), ("seed", ctypes.c_uint)]
+                ("low", P), ("step", P), ("done", P), ("hyper_dev", P), ("hyper", ctypes.c_double * 7), ("clip", P), ("seed", ctypes.c_uint)]
 
 
 _address, _dense = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
@@ -404,7 +403,7 @@ class AdamW(Adam):
 
     def _launch(self, work, dev):
         stream, capturing = _lib.current_stream(), torch.cuda.is_current_stream_capturing()
-        used, partial = 0, None
+        clip = None
         if self.max_grad_norm is not None:
             launches = lambda ps: (len(ps) + MAX_TENSORS - 1) // MAX_TENSORS + 1      # noqa: E731   (fp32 and bf16 ones apart)
             room = GRAD_SQUARE_SUMS * sum(launches(g["params"]) for g in self.param_groups)
@@ -412,14 +411,18 @@ class AdamW(Adam):
                 if capturing:
                     raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: run one eager step before capture")
                 if self._norm is None:
-                    self._norm = torch.zeros((), dtype=torch.float32, device=dev)
+                    self._factors = torch.zeros((2,), dtype=torch.float32, device=dev)          # the norm, and what the gradients are multiplied by
+                    self._norm = self._factors[0]
                 self._partial.append(torch.empty((room,), dtype=torch.float64, device=dev))
             partial = self._partial[-1].data_ptr()
-            n = c_int()
+            n, used = c_int(), 0
             for w in work:
                 for bf16, t in w[3]:
                     _lib.call("rs_grad_square_sums", t.ref, bf16, partial + 8 * used, room - used, ctypes.byref(n), stream)
                     used += n.value
+            if used:
+                _lib.call("rs_grad_norm", used, partial, self.max_grad_norm, self._factors.data_ptr(), stream)
+                clip = self._factors.data_ptr() + 4
         for gi, group, st, tables, _ in work:
             key = (float(group["lr"]), tuple(group["betas"]), group["eps"], group["weight_decay"])
             if st["key"] != key:
@@ -435,9 +438,7 @@ class AdamW(Adam):
                 if t.vals is not st["vals"]:
                     a.hyper[:], t.vals = st["vals"], st["vals"]
                 a.hyper_dev = st["hyper"].data_ptr() if capturing else None
-                a.partial, a.npartial = (partial, used) if used else (None, 0)
-                if used:
-                    a.norm, a.max_norm = self._norm.data_ptr(), self.max_grad_norm
+                a.clip = clip
                 _lib.call("rs_adamw_step", t.ref, ctypes.byref(a), stream)
 
     def _args(self, gi, st, bf16):

@@ -73,8 +73,7 @@ def test_entry_points_report_bad_arguments():
         d.update(kw)
         return ctypes.byref(optim.AdamWArgs(**d))
 
-    for a, text in [(dict(bits=16), "bits"), (dict(bits=8), "bits"), (dict(bf16=1), "low"), (dict(exp_avg=None), "null"), (dict(done=None), "null"),
-                    (dict(partial=256), "partial"), (dict(partial=256, npartial=1, norm=256, max_norm=0.0), "partial")]:
+    for a, text in [(dict(bits=16), "bits"), (dict(bits=8), "bits"), (dict(bf16=1), "low"), (dict(exp_avg=None), "null"), (dict(done=None), "null")]:
         with pytest.raises(_lib.RepSurfHipError, match=text):
             _lib.call("rs_adamw_step", listed(), args(**a), None)
     with pytest.raises(_lib.RepSurfHipError, match="null pointer"):
@@ -88,6 +87,9 @@ def test_entry_points_report_bad_arguments():
     used = ctypes.c_int()
     with pytest.raises(_lib.RepSurfHipError, match="room"):
         _lib.call("rs_grad_square_sums", listed(), 0, 256, 0, ctypes.byref(used), None)
+    for a in ((0, 256, 1.0, 256), (1, None, 1.0, 256), (1, 256, 0.0, 256), (1, 256, 1.0, None)):
+        with pytest.raises(_lib.RepSurfHipError, match="rs_grad_norm"):
+            _lib.call("rs_grad_norm", *a, None)
     with pytest.raises(_lib.RepSurfHipError, match="null"):
         _lib.call("rs_adamw_masters", listed(), None, None, None)
     for name, a in (("rs_adamw_pack", (100,) + (256,) * 6), ("rs_adamw_unpack", (100,) + (256,) * 4 + (0, 256, 256))):
