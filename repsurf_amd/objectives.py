@@ -90,9 +90,12 @@ def _desc(logits, target, ignore_index, offset):
                       None if offset is None else offset.data_ptr(), 0 if offset is None else offset.numel(), bad)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(device, name, *args):
     """an ABI call on the current stream of the tensors' device"""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         _lib.call(name, *args, _lib.current_stream())
     else:
         with torch.cuda.device(device):
@@ -101,15 +104,30 @@ def _call(device, name, *args):
 
 def _backward(ctx, logits, target, offset, work, coef, gout, skip_unit=0, out=None):
     """from the tensors as autograd hands them back (a hook may have moved them); the rows' stat lies in `work`, ctx.stat floats from its
-    start; coef: an address"""
+    start; coef: an address.  (Autograd runs this on a thread of its own, whose every line costs twice what it costs elsewhere.)"""
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    desc = ctx.desc
-    desc.logits, desc.ld, desc.target = logits.data_ptr(), max(logits.stride(0), logits.shape[1]), target.data_ptr()
-    desc.offset, desc.sequences = (None, 0) if offset is None else (offset.data_ptr(), offset.numel())
-    _call(logits.device, "rs_token_logprobs_backward", ctypes.byref(desc), work.data_ptr() + 4 * ctx.stat, coef,
-          None if gout is None else _as(gout, torch.float32).data_ptr(), skip_unit, out.data_ptr())
+    desc, at = ctx.desc, logits.data_ptr()
+    if at != desc.logits or target.data_ptr() != desc.target or (offset is not None and offset.data_ptr() != desc.offset):
+        desc.logits, desc.ld, desc.target = at, max(logits.stride(0), logits.shape[1]), target.data_ptr()
+        if offset is not None:
+            desc.offset = offset.data_ptr()
+    if gout is not None:
+        gout = (gout if gout.dtype is torch.float32 else gout.to(torch.float32)).data_ptr()
+    _call(logits.device, "rs_token_logprobs_backward", ctx.ref, work.data_ptr() + 4 * ctx.stat, coef, gout, skip_unit, out.data_ptr())
     return out
+
+
+def _once(fn):
+    """a backward pass that can be differentiated no further; the wrapper that says so is entered only where somebody builds its graph"""
+    careful = once_differentiable(fn)
+    return lambda ctx, *g: careful(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
+
+
+def _keep(ctx, desc, stat, *tensors):
+    ctx.set_materialize_grads(False)          # (no zeros for the outputs that have no gradient)
+    ctx.save_for_backward(*tensors)
+    ctx.desc, ctx.ref, ctx.stat = desc, ctypes.byref(desc), stat
 
 
 def _wanted(logits):
@@ -137,12 +155,11 @@ class _TokenLogprobs(Function):
         _call(logits.device, "rs_token_logprobs", ctypes.byref(desc), logp.data_ptr(), None, work.data_ptr() + 4 * room if grad else None,
               work.data_ptr() if room else None)
         if grad:
-            ctx.save_for_backward(logits, target, work)
-            ctx.desc, ctx.stat = desc, room
+            _keep(ctx, desc, room, logits, target, work)
         return logp
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         logits, target, work = ctx.saved_tensors
         g = _as(g, torch.float32)
@@ -178,12 +195,11 @@ class _SequenceLogprobs(Function):
     def forward(ctx, logits, target, offset, ignore_index, average, grad):
         desc, out, buf, places = _sequences(logits, target, offset, ignore_index, average)
         if grad:
-            ctx.save_for_backward(logits, target, offset, buf)
-            ctx.desc, ctx.stat = desc, places["stat"]
+            _keep(ctx, desc, places["stat"], logits, target, offset, buf)
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         logits, target, offset, buf = ctx.saved_tensors
         coef = _as(g, torch.float32) * buf[buf.numel() - offset.numel():]
@@ -206,13 +222,13 @@ class _Preference(Function):
         _call(logits.device, "rs_preference_pairs", n // 2, start + 4 * places["sums"], start + 4 * places["each"], ref.data_ptr(), beta, smoothing,
               loss.data_ptr(), rewards.data_ptr(), start + 4 * places["extra"])
         if grad:
-            ctx.save_for_backward(logits, target, offset, buf)
-            ctx.desc, ctx.stat, ctx.coef = desc, places["stat"], places["extra"]
+            _keep(ctx, desc, places["stat"], logits, target, offset, buf)
+            ctx.coef = places["extra"]
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g, _):
         logits, target, offset, buf = ctx.saved_tensors
         return (_backward(ctx, logits, target, offset, buf, buf.data_ptr() + 4 * ctx.coef, g),) + (None,) * 8
@@ -257,21 +273,23 @@ class _Policy(Function):
                        coef if held else None, stat if held else None, scratch if room else None)
         _call(logits.device, "rs_policy_loss", ctypes.byref(desc), ctypes.byref(p))
         if grad:
-            ctx.save_for_backward(logits, target, work)
-            ctx.d, ctx.desc, ctx.stat = d, desc, (stat - at) // 4
+            desc.offset, desc.sequences = None, 0           # (coef is per row, 0 for the rows behind the last sequence)
+            _keep(ctx, desc, (stat - at) // 4, logits, target, work)
+            ctx.d = d
         ctx.mark_non_differentiable(logp, stats)
         return loss, logp, stats
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g, *_):
         logits, target, work = ctx.saved_tensors
-        d, first = ctx.d, ctx.d is not None
+        d = ctx.d
+        first = d is not None
         ctx.d = None                       # handed out once: a second pass over a retained graph computes it again
-        one = head._unit.get(str(logits.device)) if head._unit else None
-        if first and ((one is not None and g.data_ptr() == one.data_ptr()) or logits.shape[0] == 0):      # loss.backward(unit_gradient(device))
-            return (d,) + (None,) * 11
-        # coef is per row, 0 for the rows behind the last sequence: no offsets
+        if first and head._unit:
+            one = head._unit.get(str(logits.device))
+            if one is not None and g.data_ptr() == one.data_ptr():          # loss.backward(unit_gradient(device))
+                return (d,) + (None,) * 11
         coef = work.data_ptr() + 4 * (ctx.stat + 2 * logits.shape[0])
         return (_backward(ctx, logits, target, None, work, coef, g, int(first), d),) + (None,) * 11
 
