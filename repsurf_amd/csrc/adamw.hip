@@ -437,23 +437,29 @@ adamw_masters_kernel(AwTable T, const short *__restrict__ low, float *__restrict
   }
 }
 
-// calls f(table, chunks) for runs of at most AW_MAX tensors
+constexpr long long AW_CHUNKS = (1LL << 24) - 1;      // workgroups of 256 threads: a launch holds fewer than 2^32 threads
+constexpr int AW_GRID = 1 << 22;
+
+// calls f(table, chunks) for runs of at most AW_MAX tensors and AW_CHUNKS chunks
 template <typename F>
 int aw_tables(const rs_adamw_list *l, const char *name, int chunk, F f) {
   RS_REQUIRE(l && l->count >= 0 && (l->count == 0 || (l->p && l->g && l->n && l->at && l->slot)), "%s: null pointer", name);
-  for (int first = 0; first < l->count; first += AW_MAX) {
+  for (int k = 0; k < l->count; ++k) {
+    RS_REQUIRE(l->p[k] && l->g[k] && l->n[k] > 0 && l->at[k] >= 0 && l->at[k] % AW_BLOCK == 0 && l->slot[k] >= 0,
+               "%s: tensor %d: null pointer, empty, or not at a multiple of %d elements", name, k, AW_BLOCK);
+    RS_REQUIRE((l->n[k] + chunk - 1) / chunk <= AW_CHUNKS, "%s: tensor %d has %lld elements, at most %lld are served", name, k, l->n[k], AW_CHUNKS * chunk);
+  }
+  for (int k = 0; k < l->count;) {
     AwTable T;
-    T.count = l->count - first < AW_MAX ? l->count - first : AW_MAX;
     long long chunks = 0;
-    for (int i = 0; i < T.count; ++i) {
-      const int k = first + i;
-      RS_REQUIRE(l->p[k] && l->g[k] && l->n[k] > 0 && l->at[k] >= 0 && l->at[k] % AW_BLOCK == 0 && l->slot[k] >= 0,
-                 "%s: tensor %d: null pointer, empty, or not at a multiple of %d elements", name, k, AW_BLOCK);
+    int i = 0;
+    for (; i < AW_MAX && k < l->count; ++i, ++k) {
+      const long long more = (l->n[k] + chunk - 1) / chunk;
+      if (chunks + more > AW_CHUNKS) break;
       T.p[i] = l->p[k]; T.g[i] = l->g[k]; T.n[i] = l->n[k]; T.at[i] = l->at[k]; T.slot[i] = l->slot[k];
-      chunks += (l->n[k] + chunk - 1) / chunk;
-      RS_REQUIRE(chunks < (1LL << 31), "%s: too many elements in one launch", name);
-      T.blk_end[i] = (int)chunks;
+      T.blk_end[i] = (int)(chunks += more);
     }
+    T.count = i;
     const int rc = f(T, (int)chunks);
     if (rc != RS_OK) return rc;
   }
@@ -523,7 +529,7 @@ extern "C" int rs_adamw_pack(long long n, const float *m, const float *v, unsign
   if (n == 0) return RS_OK;
   RS_REQUIRE(m && v && mc && vc && me && ve, "rs_adamw_pack: null pointer");
   const long long blocks = n / AW_BLOCK, wgs = (blocks + 3) / 4;
-  hipLaunchKernelGGL(adamw_pack_kernel, dim3((int)(wgs < (1 << 30) ? wgs : (1 << 30))), dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, m, v, mc, vc, me, ve);
+  hipLaunchKernelGGL(adamw_pack_kernel, dim3((int)(wgs < AW_GRID ? wgs : AW_GRID)), dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, m, v, mc, vc, me, ve);
   RS_CHECK_LAUNCH("rs_adamw_pack");
   return RS_OK;
 }
@@ -534,7 +540,7 @@ extern "C" int rs_adamw_unpack(long long n, const unsigned char *mc, const unsig
   if (n == 0) return RS_OK;
   RS_REQUIRE(m && v && mc && vc && me && ve, "rs_adamw_unpack: null pointer");
   const long long blocks = n / AW_BLOCK, wgs = (blocks + 3) / 4;
-  const dim3 grid((int)(wgs < (1 << 30) ? wgs : (1 << 30)));
+  const dim3 grid((int)(wgs < AW_GRID ? wgs : AW_GRID));
   if (out_bf16) hipLaunchKernelGGL((adamw_unpack_kernel<__bf16>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (__bf16 *)m, (__bf16 *)v);
   else hipLaunchKernelGGL((adamw_unpack_kernel<float>), grid, dim3(AW_THREADS), 0, (hipStream_t)stream, blocks, mc, vc, me, ve, (float *)m, (float *)v);
   RS_CHECK_LAUNCH("rs_adamw_unpack");

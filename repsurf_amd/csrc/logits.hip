@@ -684,7 +684,7 @@ int check_rows(const rs_logits *l, const char *name) {
   RS_REQUIRE(l && l->rows >= 0 && l->classes > 0 && l->classes <= 1 << 30 && l->ld >= l->classes && l->type >= 0 && l->type <= 2, "%s: bad size or type", name);
   RS_REQUIRE(l->sequences >= 0 && (!l->offset) == (l->sequences == 0), "%s: offsets and their number do not match", name);
   RS_REQUIRE(l->rows == 0 || (l->logits && l->target), "%s: null pointer", name);
-  RS_REQUIRE(!l->offset || l->rows < (1LL << 31), "%s: too many rows for 32-bit offsets", name);
+  RS_REQUIRE(l->rows < (1LL << 31), "%s: %lld rows (offsets and counts have 32 bits)", name, l->rows);
   return RS_OK;
 }
 Rows rows_of(const rs_logits *l) {

@@ -306,6 +306,8 @@ class AdamW(Adam):
         bits = {32 if v["exp_avg"].is_floating_point() else 8 for v in state_dict["state"].values() if "exp_avg" in v}
         if len(bits) > 1 or (bits == {8} and self.state_bits == 32):
             raise ValueError("AdamW.load_state_dict: 8-bit moments need state_bits=8 (and all of them)")
+        if any(k in v and k + "_exponent" not in v for v in state_dict["state"].values() for k in ("exp_avg", "exp_avg_sq") if 8 in bits):
+            raise ValueError("AdamW.load_state_dict: 8-bit moments without their exponents")
         if any(sg.get("amsgrad") or sg.get("maximize") for sg in state_dict["param_groups"]):
             raise ValueError("AdamW.load_state_dict: amsgrad and maximize are not offered")
         order = [list(sg["params"]) for sg in state_dict["param_groups"]]

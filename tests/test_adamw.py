@@ -54,6 +54,10 @@ def test_foreign_state_is_refused():
     with pytest.raises(ValueError, match="8-bit"):
         opt.load_state_dict({"state": {0: {"step": 1.0, "exp_avg": torch.zeros(3, dtype=torch.uint8), "exp_avg_sq": torch.zeros(3, dtype=torch.uint8)}},
                              "param_groups": groups})
+    with pytest.raises(ValueError, match="exponents"):
+        optim.AdamW(params((3,)), state_bits=8).load_state_dict(
+            {"state": {0: {"step": 1.0, "exp_avg": torch.zeros(3, dtype=torch.uint8), "exp_avg_sq": torch.zeros(3, dtype=torch.uint8)}},
+             "param_groups": groups})
     opt.load_state_dict({"state": {}, "param_groups": groups})          # a fresh torch optimizer's state dict
     assert opt.param_groups[0]["lr"] == groups[0]["lr"]
 
@@ -81,6 +85,9 @@ def test_entry_points_report_bad_arguments():
     for bad in ((ctypes.c_longlong * 1)(0), (ctypes.c_longlong * 1)(-5)):
         with pytest.raises(_lib.RepSurfHipError, match="tensor 0"):
             _lib.call("rs_adamw_step", listed(n=cast(bad)), args(), None)
+    huge = (ctypes.c_longlong * 1)(1 << 36)
+    with pytest.raises(_lib.RepSurfHipError, match="at most"):
+        _lib.call("rs_adamw_step", listed(n=cast(huge)), args(), None)
     odd = (ctypes.c_longlong * 1)(128)
     with pytest.raises(_lib.RepSurfHipError, match="multiple of 256"):
         _lib.call("rs_adamw_step", listed(at=cast(odd)), args(), None)

@@ -153,6 +153,55 @@ def test_it_resumes_from_torch_and_torch_from_it():
         assert torch.equal(back.state[p]["exp_avg"], opt.state[q]["exp_avg"]) and float(back.state[p]["step"]) == 5.0
 
 
+def test_it_loads_from_the_cpu_and_from_bf16_moments(tmp_path):
+    """a checkpoint mapped to the CPU; torch's own for bf16 parameters, whose moments are bf16"""
+    from repsurf_amd.optim import AdamW
+    a = make(SHAPES, torch.bfloat16)
+    for bits in (32, 8):
+        first = AdamW(a, state_bits=bits, seed=2, **HYPER)
+        give(a, 1)
+        first.step()
+        torch.save(first.state_dict(), tmp_path / "o.pt")
+        b = make(SHAPES, torch.bfloat16)
+        second = AdamW(b, state_bits=bits, seed=2, **HYPER)
+        second.load_state_dict(torch.load(tmp_path / "o.pt", map_location="cpu", weights_only=True))
+        for k, x in first.flat_state().items():
+            assert torch.equal(x, second.flat_state()[k])
+    b = make(SHAPES, torch.bfloat16)
+    ref = torch.optim.AdamW(b, **HYPER)
+    give(b, 1)
+    ref.step()
+    opt = AdamW(b, **HYPER)
+    opt.load_state_dict(ref.state_dict())
+    for p in b:
+        assert torch.equal(opt.state[p]["exp_avg"], ref.state[p]["exp_avg"].float())
+    assert int(opt._dev[0]["step"][0]) == 1
+
+
+def test_a_master_is_what_the_parameter_was_and_what_it_cut_off():
+    """the halves of words at the borders of the format: ties, the largest numbers, denormals, NaNs with a payload"""
+    from repsurf_amd.optim import AdamW
+    words = torch.tensor([0, 0x7FFF, 0x8000, 0x8001, 0xFFFF, 0x10000, 0x3F808000, 0x3F80FFFF, 0x3F818000, 0x7F7FFFFF, 0x7F7F8000, 0x7F800000, 0x1, 0x00800000], dtype=torch.int64)
+    words = torch.cat([words, words + 0x80000000])
+    x = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32).view(torch.float32)
+    p = torch.nn.Parameter(torch.zeros(len(x), dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    opt = AdamW([p], lr=0.0, weight_decay=0.0)
+    opt.step()
+    bits = words + 0x8000
+    with torch.no_grad():                                   # as a step would have left them
+        up = (bits >> 16) & 0xFFFF
+        p.view(torch.int16).copy_(torch.where(up >= 1 << 15, up - (1 << 16), up).to(torch.int16))
+        low = words & 0xFFFF
+        opt.flat_state()["low"][:len(x)] = torch.where(low >= 1 << 15, low - (1 << 16), low).to(torch.int16).cuda()
+    master = opt.unpack_state()["master"][:len(x)].cpu()
+    assert torch.equal(master.view(torch.int32), x.view(torch.int32))
+    opt.step()                                              # a rate of nothing: the same words again
+    again = opt.unpack_state()["master"][:len(x)].cpu()
+    finite = torch.isfinite(x)
+    assert torch.equal(again.view(torch.int32)[finite], x.view(torch.int32)[finite]) and torch.isinf(again[~finite]).sum() + torch.isnan(again[~finite]).sum() == (~finite).sum()
+
+
 def test_bf16_parameters_keep_their_masters():
     """200 steps of 1e-4 each on values near 1: bf16's spacing there is 2^-7, so without a master nothing would move"""
     from repsurf_amd.optim import AdamW

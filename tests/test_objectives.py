@@ -38,7 +38,7 @@ def test_entry_points_report_bad_arguments():
         return ctypes.byref(O.LogitsDesc(**d))
 
     for bad in (dict(rows=-1), dict(classes=0), dict(ld=7), dict(type=3), dict(offset=256), dict(sequences=2), dict(logits=None), dict(target=None),
-                dict(classes=(1 << 30) + 1, ld=1 << 31), dict(rows=1 << 31, offset=256, sequences=1)):
+                dict(classes=(1 << 30) + 1, ld=1 << 31), dict(rows=1 << 31, offset=256, sequences=1), dict(rows=1 << 31)):
         with pytest.raises(_lib.RepSurfHipError, match="rs_token_logprobs"):
             _lib.call("rs_token_logprobs", rows(**bad), 256, None, None, None, None)
         with pytest.raises(_lib.RepSurfHipError):
