@@ -7,6 +7,9 @@ LIBDIR := repsurf_amd/lib
 # operation by operation; fused multiply-adds appear only where written (rs_fma).
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off \
             -fhip-fp32-correctly-rounded-divide-sqrt -munsafe-fp-atomics -Wall -Wno-unused-function
+# No packed-fp32 instructions anywhere: some of their forms give other results beside another kernel's MFMAs (see below).  At no cost: the
+# classification step 1.218 ms with and 1.217 ms without them, the segmentation step 3.314 and 3.319 ms (runs of each in turn, one GPU).
+HIPFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 SRCS := $(CSRC)/rs_lib.cpp $(CSRC)/fps.hip $(CSRC)/ballquery.hip $(CSRC)/knn_umbrella.hip $(CSRC)/knn_wide.hip \
         $(CSRC)/group.hip $(CSRC)/interp.hip $(CSRC)/seg_geom.hip $(CSRC)/scene_knn.hip $(CSRC)/grid_knn.hip $(CSRC)/mlp.hip $(CSRC)/umbrella_mlp.hip $(CSRC)/umbrella_mfma.hip $(CSRC)/head.hip $(CSRC)/adam.hip $(CSRC)/adamw.hip $(CSRC)/logits.hip
 OBJS := $(patsubst $(CSRC)/%,build/%.o,$(SRCS)) build/mlp_bf16.hip.o build/mlp_sb.hip.o build/mlp_split.hip.o
@@ -20,9 +23,6 @@ OBJS := $(patsubst $(CSRC)/%,build/%.o,$(SRCS)) build/mlp_bf16.hip.o build/mlp_s
 # arithmetic is the same IEEE operations either way.
 GEOM_TUS := fps ballquery knn_umbrella knn_wide group interp seg_geom scene_knn grid_knn umbrella_mlp head adam adamw logits
 $(foreach t,$(GEOM_TUS),$(eval build/$(t).hip.o: HIPFLAGS += -fno-slp-vectorize -fno-vectorize))
-# ... and these without packed-fp32 instructions at all
-NOPK := -Xclang -target-feature -Xclang -packed-fp32-ops
-build/adamw.hip.o build/logits.hip.o: HIPFLAGS += $(NOPK)
 
 all: $(LIBDIR)/librepsurf_hip.so oracle
 

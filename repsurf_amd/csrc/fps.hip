@@ -137,9 +137,8 @@ fps_reg_kernel(int n_arg, int m_arg, const float *__restrict__ xyz, const int *_
     if (tid == 0) out[it] = cur + seg.idx_base;
     if (it == m - 1) break;
 
-    // distance update + per-lane max.  Two points per instruction where the lane owns an even number of them:
-    // v_pk_add_f32 / v_pk_mul_f32 round each half exactly like the scalar forms (no contraction), and the update is
-    // the longest VALU stretch of a pick.
+    // distance update + per-lane max, the longest VALU stretch of a pick: two points at a time where the lane owns an even number of them
+    // (as two scalar operations each: the library is built without packed-fp32 instructions; the rounding is the same, no contraction).
     int lmax = (int)0x80000000;
     if constexpr (PPT % 2 == 0) {
       typedef float v2f __attribute__((ext_vector_type(2)));
