@@ -199,8 +199,10 @@ struct AwBlocks {
         if constexpr (BITS == 8) { mi[i] = aw_decode_m(aw_get(mc[u], i), em[u]); vi[i] = aw_decode_v(aw_get(vc[u], i), ev[u]); }
         else { mi[i] = aw_get(m[u], i); vi[i] = aw_get(v[u], i); }
         gi *= S.clip;
-        mi[i] = rs_fma(gi - mi[i], S.omb1, mi[i]);
-        vi[i] = rs_fma(S.omb2 * gi, gi, vi[i] * S.b2);
+        // Each operation of the moments is rounded by itself, as the formula is written: an 8-bit moment next to a border of its grid then falls
+        // to the side that the elementary operations choose, and a step larger or smaller by an eighth does not hang on a fused rounding.
+        mi[i] = mi[i] + (gi - mi[i]) * S.omb1;
+        vi[i] = vi[i] * S.b2 + (S.omb2 * gi) * gi;
         // The device's own root and reciprocal, each off by one unit: the correctly rounded ones are 25 instructions for an error that lr
         // scales away.  The root takes denormals as zero, so v is raised to the smallest normal number (1e-19 beside eps).
         const float root = __builtin_amdgcn_sqrtf(fmaxf(vi[i], 1.17549435e-38f));
@@ -298,8 +300,8 @@ adamw_kernel(AwTable T, AwArgs A) {
 }
 
 // ---- the gradients' common norm -------------------------------------------------------------------------------------
-// partial[b] = sum of the squares of workgroup b's chunks.  A lane's 32 squares of a chunk are added in fp32, everything above in fp64, in
-// an order that the sizes fix.
+// partial[b] = sum of the squares of workgroup b's chunks, in fp64 and in an order that the sizes fix: the norm is the correctly rounded one but
+// for a few cases in a thousand million, and the factor that every gradient is multiplied by hangs on no order.
 template <bool BF16>
 __global__ void __launch_bounds__(AW_THREADS)
 grad_sq_kernel(AwTable T, double *__restrict__ partial) {
@@ -313,31 +315,32 @@ grad_sq_kernel(AwTable T, double *__restrict__ partial) {
     const int ti = find(c);
     const long long left = T.n[ti] - (long long)(c - (ti ? T.blk_end[ti - 1] : 0)) * AW_SQ_CHUNK;
     const PT *__restrict__ g = (const PT *)T.g[ti] + (T.n[ti] - left);
-    float a = 0.f;
     if (left >= AW_SQ_CHUNK) {
       unsigned w[U][4];
 #pragma unroll
       for (int u = 0; u < U; ++u) __builtin_memcpy(w[u], g + (u * AW_THREADS + (int)threadIdx.x) * E, 16);
+      double a[2] = {0.0, 0.0};
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float t = 0.f;
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (BF16) {
-            const float x = __uint_as_float(w[u][i] << 16), y = __uint_as_float(w[u][i] & 0xFFFF0000u);
-            t = rs_fma(x, x, rs_fma(y, y, t));
-          } else t = rs_fma(__uint_as_float(w[u][i]), __uint_as_float(w[u][i]), t);
+            const double x = (double)__uint_as_float(w[u][i] << 16), y = (double)__uint_as_float(w[u][i] & 0xFFFF0000u);
+            a[0] = fma(x, x, a[0]);
+            a[1] = fma(y, y, a[1]);
+          } else {
+            const double x = (double)__uint_as_float(w[u][i]);
+            a[i & 1] = fma(x, x, a[i & 1]);
+          }
         }
-        a += t;
-      }
+      s += a[0] + a[1];
     } else {
       for (int e = (int)threadIdx.x; e < (int)left; e += AW_THREADS) {
         float x;
         if constexpr (BF16) x = __uint_as_float((unsigned)g[e] << 16); else x = g[e];
-        a = rs_fma(x, x, a);
+        s = fma((double)x, (double)x, s);
       }
     }
-    s += (double)a;
   }
   red[threadIdx.x] = s;
   __syncthreads();
@@ -362,7 +365,7 @@ grad_norm_kernel(int n, const double *__restrict__ partial, float max_norm, floa
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    const float norm = (float)sqrt(red[0]), c = max_norm / (norm + 1e-6f);
+    const float norm = (float)sqrt(red[0]), c = (1.f / (norm + 1e-6f)) * max_norm;      // (a quotient by a tensor is its reciprocal's product there)
     out[0] = norm;
     out[1] = c > 1.f ? 1.f : c;
   }

@@ -1,7 +1,7 @@
 """repsurf_amd.optim.AdamW (csrc/adamw.hip) against its formulas in 64 bits.
 
-Tolerances.  u = 2^-24, half a step of fp32.  One update rounds m three times (difference, product in the fma's one rounding, the constant
-1 - b1) and v four times, each by at most u of the largest term; the moments contract, so over k steps |dm| <= 4 k u max|m, g|, and
+Tolerances.  u = 2^-24, half a step of fp32.  One update rounds m four times (the constant 1 - b1, difference, product, sum) and v six times
+(two constants, three products, the sum; all but three of them on the small term), each by at most u of the largest term; the moments contract, so over k steps |dm| <= 4 k u max|m, g|, and
 |dv| <= 5 k u max(v, g^2).  The update's ratio is then off by at most (4 + 2.5 + 9) k u relative -- the square root halves v's error; the device's
 root and reciprocal (2 u each), the sum, the product, the step size and the bias corrections add nine -- and p by k (3 u |p| + 16 k u lr r), r the largest
 ratio seen: the constant 1 - lr wd, its product with p and the sum are three roundings of at most u |p| each."""
@@ -275,6 +275,34 @@ def test_8_bits_against_the_format_in_64_bits(dtype):
         state = got
 
 
+@pytest.mark.parametrize("clip", [None, 0.05])
+def test_8_bit_moments_are_those_of_the_elementary_operations(clip):
+    """Two steps against torch's own fp32 operations and the rounding in 64 bits, on a million elements: no moment differs.  Both sides
+    round the same values the same way but in the grid's linear part, where the kernel's word has 20 bits below a step: one element in 2^20
+    of those there, none expected here."""
+    from repsurf_amd.optim import AdamW
+    n = 1 << 20
+    g = torch.Generator().manual_seed(7)
+    p = torch.nn.Parameter(torch.randn(n, generator=g).cuda())
+    opt = AdamW([p], state_bits=8, seed=4, max_grad_norm=clip, **HYPER)
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    for t in (1, 2, 3):
+        p.grad = (torch.randn(n, generator=g) * 1e-3).cuda()
+        x = p.grad
+        if clip:
+            norm = x.double().square().sum().sqrt().float()
+            x = x * torch.clamp(clip / (norm + 1e-6), max=1.0)
+        m = m + (x - m) * (1 - 0.9)
+        v = v * 0.999 + (1 - 0.999) * x * x
+        opt.step()
+        dm, dv = O.dither(4, t, 0, n // 256)
+        m, v = (torch.from_numpy(O.quantise(np64(y).reshape(-1, 256), s, d)[0].reshape(-1)).float().cuda() for y, s, d in ((m, True, dm), (v, False, dv)))
+        got = opt.unpack_state()
+        assert int((got["exp_avg"] != m).sum()) == 0 and int((got["exp_avg_sq"] != v).sum()) == 0, t
+        if clip:
+            assert torch.equal(opt.grad_norm, norm)
+
+
 def test_8_bits_decay_a_second_moment():
     """one large gradient, then none: rounded to nearest, b2 v would stay v for ever"""
     from repsurf_amd.optim import AdamW
@@ -356,8 +384,7 @@ def test_8_bit_state_dicts(tmp_path):
 @pytest.mark.parametrize("bits,dtype", [(32, torch.float32), (8, torch.bfloat16)])
 @pytest.mark.parametrize("bound", [1.0, 1e6])
 def test_clipping_by_the_common_norm(bits, dtype, bound):
-    """The norm: squares and sums of at most 32 in fp32, one after the other at a tensor's end: 32 roundings of u, half of them in the root; fp64
-    above, one rounding: 17 u."""
+    """The norm is summed in fp64 and rounded once."""
     from repsurf_amd.optim import AdamW
     ps = make(SHAPES * 9, dtype)
     give(ps, 3)
@@ -366,7 +393,7 @@ def test_clipping_by_the_common_norm(bits, dtype, bound):
     before = [p.detach().clone() for p in ps]
     grads = [p.grad.clone() for p in ps]
     clipped.step()
-    assert abs(float(clipped.grad_norm) / want - 1) <= 17 * U
+    assert abs(float(clipped.grad_norm) / want - 1) <= 1.001 * U
     assert all(torch.equal(p.grad, g) for p, g in zip(ps, grads))
     m = np64(clipped.unpack_state()["exp_avg"])
     at, c = 0, min(1.0, bound / (want + 1e-6))
