@@ -16,6 +16,12 @@
 //
 // bf16 parameters: the fp32 master's upper half, rounded, IS the parameter; `low` keeps what the rounding cut off (16 signed bits), so
 // master bits = (parameter bits << 16) + low and a parameter that is written from outside moves its master with it.
+//
+// Bound by memory: every value is read and written once.  A workgroup takes one chunk of 2048 elements of one tensor, all of its loads in
+// flight at once; workgroups that loop over chunks (2048 of them) were 8..16 % slower, 4096 elements a chunk no faster.  Measured: 100.7 M fp32
+// parameters with fp32 moments 498 us (28 bytes each, 5.7 TB/s), 59.6 M bf16 parameters 272 us (26 bytes, 5.7 TB/s), 268 M fp32 parameters
+// with 8-bit moments 776 us (16 bytes, 5.5 TB/s), 100.7 M bf16 parameters with 8-bit moments 248 us (14 bytes, 5.7 TB/s); 1.48 M in 67
+// tensors 9.3 us, most of it the launch, two dependent reads and the counting of finished workgroups (1.2 us).
 #include "rs_common.h"
 #include <math.h>
 
@@ -300,6 +306,7 @@ adamw_kernel(AwTable T, AwArgs A) {
 }
 
 // ---- the gradients' common norm -------------------------------------------------------------------------------------
+// Bound by memory: 100.7 M fp32 gradients 101 us = 4.0 TB/s (what the step before wrote is still on its way to memory), bf16 45 us.
 // partial[b] = sum of the squares of workgroup b's chunks, in fp64 and in an order that the sizes fix: the norm is the correctly rounded one but
 // for a few cases in a thousand million, and the factor that every gradient is multiplied by hangs on no order.
 template <bool BF16>
@@ -371,7 +378,7 @@ grad_norm_kernel(int n, const double *__restrict__ partial, float max_norm, floa
   }
 }
 
-// ---- 8-bit moments <-> values, flat ---------------------------------------------------------------------------------
+// ---- 8-bit moments <-> values, flat (bound by memory: 268 M pairs to bf16 276 us = 5.8 TB/s) ---------------------------------------------------------------------------------
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_pack_kernel(long long blocks, const float *__restrict__ m, const float *__restrict__ v, unsigned char *__restrict__ mc,
                   unsigned char *__restrict__ vc, unsigned char *__restrict__ me, unsigned char *__restrict__ ve) {

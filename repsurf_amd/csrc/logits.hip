@@ -271,12 +271,16 @@ __device__ __forceinline__ void lg_partial(const Policy &P, const double *add, i
 
 // Rows of up to 4096 classes: LANES neighbouring lanes hold a row in NV vectors of 8 per lane; one read, one write.  A team takes SUB rows
 // before the fp64 steps, which its first SUB lanes then do for a row each: with 13 classes (2 lanes, 2 rows) every lane of a wave works
-// on a row of its own.
+// on a row of its own.  The policy loss is bound by those steps (some 300 instructions in fp64) and by the registers that its rows stay
+// in; four waves per SIMD and SUB * NV = 4 measured best (SUB * NV = 8 with two waves: 13..18 % slower).  Against a workgroup per row
+// (long_kernel): 2048 classes 192 against 404 us, 4096 191 against 239 (65536 and 32768 rows in bf16), so the border is the 8 vectors
+// that a lane can hold.  Measured: policy loss, fp32, 65536 x 2048 247 us = 4.3 TB/s, 1048576 x 40 173 us; backward 2097152 x 13 96 us =
+// 2.3 TB/s (rows of 52 bytes, two lanes each); log-probabilities 32768 x 4096 in bf16 46 us = 5.8 TB/s.
 template <typename T, int MODE, int LANES, int NV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, MODE == LG_POLICY ? 4 : 1)
 short_kernel(Rows R, Policy P, Outs O) {
   constexpr int TEAMS = 256 / LANES;
-  constexpr int ROOM = MODE == LG_POLICY ? (8 / NV > 0 ? 8 / NV : 1) : 1, SUB = LANES < ROOM ? LANES : ROOM;
+  constexpr int ROOM = MODE == LG_POLICY && NV < 4 ? 4 / NV : 1, SUB = LANES < ROOM ? LANES : ROOM;
   const float up = MODE == LG_BACK && O.up ? *O.up : 1.f;
   if (MODE == LG_BACK && O.skip_unit && up == 1.f) return;
   const int team = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES, V = R.classes;
@@ -378,6 +382,10 @@ __device__ __forceinline__ int lg_head(const T *z, int V) {
   return n < V ? n : V;
 }
 
+// Bound by memory: policy loss in bf16 8192 x 32768 240 us, 8192 x 65536 444 us, 8192 x 50001 360 us (4.5..4.8 TB/s), fp32 8192 x 32768 429 us
+// (5.0); log-probabilities 8192 x 65536 in bf16 180 us = 5.9 TB/s.  256 threads leave room for two or three rows on a CU, whose loads, sums
+// and stores overlap (1024 threads, one row: 2.0..2.8 TB/s); at 131072 classes one row is all that fits (3.9 TB/s).  Held against read twice
+// (HELD false, 262144 classes: 3.4 TB/s), a row costs a third less traffic.
 // (WAVES per SIMD bound the registers: left alone, the compiler interleaves the steps until two waves are all that fits)
 template <typename T, int MODE, int THREADS, int NV, bool HELD, int WAVES>
 __global__ void __launch_bounds__(THREADS, WAVES)
@@ -501,7 +509,8 @@ long_kernel(Rows R, Policy P, Outs O) {
   if (MODE == LG_POLICY) lg_partial<THREADS>(P, add, (int)blockIdx.x);
 }
 
-// backward pass of long rows: a workgroup takes 256 * 8 * NV logits of a row at a time, whatever row they are of
+// backward pass of long rows: a workgroup takes 256 * 8 * NV logits of a row at a time, whatever row they are of.  Bound by memory: 8192 x
+// 65536 in bf16 379 us = 5.7 TB/s, fp32 8192 x 32768 389 us = 5.5 TB/s
 template <typename T, int NV>
 __global__ void __launch_bounds__(256, 7)
 long_back_kernel(Rows R, Outs O, int parts) {
@@ -538,7 +547,8 @@ long_back_kernel(Rows R, Outs O, int parts) {
   }
 }
 
-// Few long rows: a row in `parts` pieces, (M, s) of each ...
+// Few long rows: a row in `parts` pieces, (M, s) of each ...  (one row of 100001 classes in bf16: 3.5 + 2.1 us, against 13.7 us by one
+// workgroup; the launches' own time bounds both)
 template <typename T, int NV>
 __global__ void __launch_bounds__(256)
 part_kernel(Rows R, int parts, int piece, float *__restrict__ part_m, double *__restrict__ part_s) {
@@ -711,7 +721,7 @@ int parts_of(const rs_logits *l) {
 template <typename T, int MODE>
 int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &O, hipStream_t st) {
   const int V = R.classes;
-#define LG_RUN_SHORT(L, N) { const int sub = MODE != LG_POLICY ? 1 : L < 8 / N ? L : (8 / N), per = 256 / L * sub, g = lesser((R.rows + per - 1) / per, LG_GRID); hipLaunchKernelGGL((short_kernel<T, MODE, L, N>), dim3(g), dim3(256), 0, st, R, P, O); return g; }
+#define LG_RUN_SHORT(L, N) { const int room = MODE == LG_POLICY && N < 4 ? 4 / N : 1, per = 256 / L * (L < room ? L : room), g = lesser((R.rows + per - 1) / per, LG_GRID); hipLaunchKernelGGL((short_kernel<T, MODE, L, N>), dim3(g), dim3(256), 0, st, R, P, O); return g; }
   if (V <= 16) LG_RUN_SHORT(2, 1)
   if (V <= 32) LG_RUN_SHORT(4, 1)
   if (V <= 64) LG_RUN_SHORT(8, 1)
