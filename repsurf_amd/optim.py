@@ -140,7 +140,7 @@ class AdamWArgs(ctypes.Structure):           # rs_adamw_args
                 ("low", P), ("step", P), ("done", P), ("hyper_dev", P), ("hyper", ctypes.c_double * 7), ("clip", P), ("seed", ctypes.c_uint)]
 
 
-_address, _dense = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_address, _dense, _size = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
 
 
 class _Table:
@@ -216,7 +216,7 @@ class AdamW(Adam):
             if any(p.dtype == torch.bfloat16 for p in params):
                 flat["low"] = new(end, torch.int16)
             st = dict(hyper=new(7, torch.float64), host=None, step=new(len(params), torch.int32), done=new(DONE, torch.int32),
-                      flat=flat, at=at, end=end, ids=[id(p) for p in params], plan=None, tables=None, key=None, vals=None)
+                      flat=flat, at=at, end=end, sizes=[p.numel() for p in params], ids=[id(p) for p in params], plan=None, tables=None, key=None, vals=None)
             self._dev[gi] = st
             for p, a in zip(params, at):
                 self._views(st, p, a)
@@ -355,7 +355,8 @@ class AdamW(Adam):
         """the group's lists (fp32, bf16), rebuilt when an address changed since the last step"""
         grads = [p.grad for p in params]
         some = [g for g in grads if g is not None]
-        plan = (list(map(_address, params)), list(map(_address, some)), len(some) == len(params) or [g is None for g in grads])
+        plan = (list(map(_address, params)), list(map(_address, some)), list(map(_size, params)),          # (a gradient has its parameter's size)
+                len(some) == len(params) or [g is None for g in grads])
         if plan == st["plan"] and all(map(_dense, some)) and all(map(_dense, params)):
             return st["tables"], None
         rows, keep, seen = ([], []), [], set()
@@ -363,6 +364,8 @@ class AdamW(Adam):
             if g is None or p.numel() == 0:
                 continue
             self._check_param(p, st["step"].device)
+            if p.numel() != st["sizes"][i] or g.shape != p.shape:
+                raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: a parameter has another size than its state or its gradient")
             if g.layout != torch.strided or g.dtype != p.dtype:
                 raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: gradients must be dense and of their parameter's type")
             if p.data_ptr() in seen:

@@ -472,6 +472,18 @@ def test_refusals_on_the_device():
     q.grad = torch.zeros(8, device="cuda")
     opt = AdamW([q])
     opt.step()
+    room = torch.zeros(600, device="cuda")
+    q.data = room                                            # larger than the state that was made for it
+    with pytest.raises(_lib.RepSurfHipError, match="another size"):
+        opt.step()
+    q.grad = None
+    q.grad = torch.zeros(600, device="cuda")
+    with pytest.raises(_lib.RepSurfHipError, match="another size"):
+        opt.step()
+    q.data = room[:8]
+    q.grad = None
+    q.grad = torch.zeros(8, device="cuda")
+    opt.step()
     opt.param_groups[0]["params"] = [torch.nn.Parameter(torch.zeros(8, device="cuda"))]
     opt.param_groups[0]["params"][0].grad = torch.zeros(8, device="cuda")
     with pytest.raises(_lib.RepSurfHipError, match="changed"):
@@ -543,3 +555,63 @@ def test_the_training_loop_step_takes_it(bits):
         y = eopt.unpack_state()[k]
         assert (x - y).norm() / y.norm() < (1e-2 if bits == 32 else 0.125), k
     step.close()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_ragged_segmentation_step_takes_it(bits):
+    """graph.RaggedSegStep, two network graphs that share the optimizer's state, clipped: against the same step launched eagerly.  The
+    first loss is the eager one bit for bit, the second to what the gradients' atomics leave of one update (the bound of the same
+    comparison with Adam, test_seg_gpu.py)."""
+    from repsurf_amd.graph import RaggedSegStep
+    from repsurf_amd.head import CrossEntropyLoss
+    from repsurf_amd.optim import AdamW
+    from tests.test_seg_gpu import _ragged_batches, _seg_model, subproject
+    _, batches, labels = _ragged_batches()
+    crit = CrossEntropyLoss(ignore_index=255)
+    with subproject("segmentation"):
+        base = _seg_model()
+        base.surface_constructor.random_inv = False
+        runs = []
+        for capture in (True, False):
+            model = copy.deepcopy(base)
+            opt = AdamW(model.parameters(), state_bits=bits, max_grad_norm=1.0, seed=2, **HYPER)
+            step = RaggedSegStep(model, crit, opt, batches[0], labels[0], capacity=4 * 1024, capture=capture)
+            losses, norms = [], []
+            for s in range(4):
+                losses.append(step(batches[(s + 1) % 4], labels[(s + 1) % 4]).item())
+                torch.cuda.synchronize()
+                norms.append(float(opt.grad_norm))
+            assert [int(t) for t in opt._dev[0]["step"]] == [4] * len(opt.param_groups[0]["params"])
+            step.close()
+            runs.append((losses, norms))
+        (l1, n1), (l0, n0) = runs
+        assert l1[0] == l0[0] and abs(l1[1] - l0[1]) <= 1e-5 and np.isfinite(l1).all(), (l1, l0)
+        assert abs(n1[0] / n0[0] - 1) <= 1e-4 and np.isfinite(n1).all()
+
+
+def test_a_policy_step_of_the_segmentation_network_as_one_graph():
+    """scores by the acting network, then network, policy loss, backward, norm and update captured by graph.RaggedSegStep with the loss as its
+    criterion; padding rows carry the ignored label.  Against the eager loop of the same calls."""
+    from repsurf_amd import objectives
+    from repsurf_amd.graph import RaggedSegStep
+    from repsurf_amd.optim import AdamW
+    from tests.test_seg_gpu import _ragged_batches, _seg_model, subproject
+    _, batches, labels = _ragged_batches()
+    with subproject("segmentation"):
+        base = _seg_model()
+        base.surface_constructor.random_inv = False
+        runs = []
+        for capture in (True, False):
+            model = copy.deepcopy(base)
+            old = torch.full((4 * 1024,), -2.5, device="cuda")
+            adv = torch.randn(4 * 1024, generator=torch.Generator().manual_seed(1)).cuda()
+
+            def crit(pred, target):
+                rows = pred.shape[0]
+                return objectives.policy_loss(pred, target, old[:rows], adv[:rows], kl_coef=0.1, ref_logp=old[:rows], ignore_index=255).loss
+
+            opt = AdamW(model.parameters(), max_grad_norm=1.0, **HYPER)
+            step = RaggedSegStep(model, crit, opt, batches[0], labels[0], capacity=4 * 1024, capture=capture, ignore_index=255)
+            runs.append([step(batches[(s + 1) % 4], labels[(s + 1) % 4]).item() for s in range(4)])
+            step.close()
+        assert runs[0][0] == runs[1][0] and abs(runs[0][1] - runs[1][1]) <= 1e-4 * max(1.0, abs(runs[1][1])) and np.isfinite(runs[0]).all(), runs
