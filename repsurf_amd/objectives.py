@@ -106,7 +106,7 @@ def _backward(ctx, logits, target, offset, work, coef, gout, skip_unit=0, out=No
     """from the tensors as autograd hands them back (a hook may have moved them); the rows' stat lies in `work`, ctx.stat floats from its
     start; coef: an address.  (Autograd runs this on a thread of its own, whose every line costs twice what it costs elsewhere.)"""
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits)          # (contiguous also where the logits have a pitch)
     desc, at = ctx.desc, logits.data_ptr()
     if at != desc.logits or target.data_ptr() != desc.target or (offset is not None and offset.data_ptr() != desc.offset):
         desc.logits, desc.ld, desc.target = at, max(logits.stride(0), logits.shape[1]), target.data_ptr()
@@ -132,6 +132,13 @@ def _keep(ctx, desc, stat, *tensors):
 
 def _wanted(logits):
     return logits.requires_grad and torch.is_grad_enabled()
+
+
+def _run(function, logits, *args):
+    """a Function whose last argument says whether a gradient is wanted; scoring goes past autograd"""
+    if _wanted(logits):
+        return function.apply(logits, *args, True)
+    return function.forward(None, logits.detach(), *args, False)
 
 
 def _new(logits, *shape, dtype=torch.float32):
@@ -170,7 +177,7 @@ def token_logprobs(logits, target, ignore_index=-100):
     """logits (rows, classes), target (rows,) -> (rows,) fp32: log softmax(logits)[target], 0 for rows that do not count.  Reads the logits once;
     differentiable in them."""
     logits, target, _ = _logits(logits, target, None)
-    return _TokenLogprobs.apply(logits, target, ignore_index, _wanted(logits))
+    return _run(_TokenLogprobs, logits, target, ignore_index)
 
 
 def _sequences(logits, target, offset, ignore_index, average, extra=0):
@@ -210,7 +217,7 @@ def sequence_logprobs(logits, target, offset, ignore_index=-100, average=False):
     """(B,) fp32: the sum of token_logprobs over every sequence of a packed batch, or (average) their mean over the rows that count; 0 for
     a sequence without any.  Differentiable in the logits."""
     logits, target, offset = _logits(logits, target, offset)
-    return _SequenceLogprobs.apply(logits, target, offset, ignore_index, average, _wanted(logits))
+    return _run(_SequenceLogprobs, logits, target, offset, ignore_index, average)
 
 
 class _Preference(Function):
@@ -255,17 +262,17 @@ class _Policy(Function):
     @staticmethod
     def forward(ctx, logits, target, old, adv, ref, offset, low, high, kl_coef, token_mean, ignore_index, grad):
         rows = logits.shape[0]
-        loss, stats, logp = _new(logits), _new(logits, 2), _new(logits, rows)
+        loss, stats, logp = old.new_empty(()), old.new_empty(2), old.new_empty(rows)
         partial = 3 * min(rows, POLICY_GROUPS)
         room, counts = _scratch_floats(logits), POLICY_COUNTS * (1 if token_mean else offset.numel())
         # one buffer: partial sums (fp64), scratch, counts, then the rows' stat (pairs: at an even place) and coef
-        work = _new(logits, 2 * partial + room + counts + (3 * rows if grad else 0))
+        work = old.new_empty(2 * partial + room + counts + (3 * rows if grad else 0))
         at = work.data_ptr()
         scratch = at + 8 * partial
         count_at = scratch + 4 * room
         stat = count_at + 4 * counts
         coef = stat + 8 * rows
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+        d = torch.empty_like(logits) if grad else None
         held = grad and rows > 0
         desc = _desc(logits, target, ignore_index, offset)
         p = PolicyDesc(old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr(), int(adv.dim() == 2), int(token_mean), low, high, kl_coef,

@@ -505,3 +505,26 @@ def test_a_policy_update_of_a_point_classifier():
         losses.append(float(out.loss.detach()))
     assert torch.isfinite(torch.tensor(losses)).all() and torch.isfinite(lin.weight).all() and float(opt.grad_norm) > 0
     assert (out.logp - old).abs().max() > 0          # the second epoch's policy is another one
+
+
+def test_gradients_of_pitched_logits_are_dense():
+    """|x - M| stays below 7 and D below 3 on normal numbers: (3 * 7 + 12 + 3 * 3) u = 42 u of a p below 0.9; the coefficient exp(log p + 50) adds
+    the error of its exponent, (3 * 3 + 6) u, and its rounding"""
+    from repsurf_amd import objectives
+    whole = torch.randn(20, 40, device="cuda")
+    for z in (whole[:, :13], whole[3:4, :13], whole[:, 5:6], whole[::2, :13], whole[:13, :20].t()):
+        z = z.detach().requires_grad_(True)
+        rows = z.shape[0]
+        y = torch.zeros(rows, dtype=torch.long, device="cuda")
+        zero = torch.zeros(rows, device="cuda")
+        want = torch.zeros(rows, z.shape[1], dtype=torch.float64)
+        want[:, 0] = 1
+        want = (want - torch.softmax(z.detach().double().cpu(), 1))
+        for f, scale in ((lambda: objectives.token_logprobs(z, y).sum(), 1.0), (lambda: objectives.policy_loss(z, y, zero - 50, zero + 1, clip=(1, 1e30)).loss, None)):
+            g, = torch.autograd.grad(f(), z)
+            assert g.shape == z.shape
+            if scale:
+                assert (g.double().cpu() - want).abs().max() <= 40 * U
+            else:                                    # -r A averaged: every row's coefficient is -exp(log p + 50) / rows
+                c = -torch.exp(torch.log_softmax(z.detach().double().cpu(), 1)[:, :1] + 50) / rows
+                assert ((g.double().cpu() - c * want).abs() <= 60 * U * c.abs()).all()
