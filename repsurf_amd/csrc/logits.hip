@@ -746,8 +746,16 @@ int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &
 #define LG_RUN_LONG(TH, N, H, WV) { const int g = lesser(R.rows, MODE == LG_POLICY ? RS_POLICY_GROUPS : LG_LONG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H, WV>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
     if constexpr (MODE == LG_POLICY) {       // (without a gradient too: the loss has the same bits either way)
       constexpr int K = sizeof(T) / 2;       // 8 logits: 4 or 8 registers of a thread
-      if (V < 10240) LG_RUN_LONG(256, 4, true, K == 1 ? 5 : 4)
-      if (V < 18432) LG_RUN_LONG(256, 8, true, K == 1 ? 4 : 3)
+      // (in 16 bits 128 threads to a row while 16 steps hold it: two waves share its fp64 steps and barriers, not four.  32768 x 5000 210 us
+      // against 272, 16384 x 8192 137 against 155, 16384 x 16000 234 against 248; 8192 x 32768 223 against 217)
+      if constexpr (K == 1) {
+        if (V < 9216) LG_RUN_LONG(128, 8, true, 5)
+        if (V < 17408) LG_RUN_LONG(128, 16, true, 4)
+      } else {
+        if (V < 5120) LG_RUN_LONG(128, 4, true, 5)        // 16384 x 5000 158 us against 169; with 8 steps 16384 x 8192 229 against 222
+        if (V < 10240) LG_RUN_LONG(256, 4, true, 4)
+        if (V < 18432) LG_RUN_LONG(256, 8, true, 3)
+      }
       if (V < 34816) LG_RUN_LONG(256, 16, true, K == 1 ? 3 : 2)
       if constexpr (K == 1) {
         if (V < 51200) LG_RUN_LONG(256, 24, true, 3)

@@ -224,6 +224,48 @@ def test_policy_loss(lengths, behind, classes, dtype, reduction, use_ref, clip):
     assert not still.loss.requires_grad and all(torch.equal(a, b) for a, b in zip(still, got))      # the same bits, with a gradient or without
 
 
+@pytest.mark.parametrize("classes", [8, 16, 31, 64, 127, 250, 512, 1023, 2047, 4095, 4097, 5119, 5121, 9215, 9217, 10239, 16384, 17409, 18433, 33000, 34816, 50001, 51201,
+                                     67583, 69633, 131071, 135169])
+@pytest.mark.parametrize("dtype", list(HALF))
+def test_policy_loss_at_every_length_of_row(classes, dtype):
+    """260 rows (more than the few that are cut over many workgroups), on both sides of the lengths where the kernels change: every
+    log-probability in 64 bits on the device, the gradients of six rows as above"""
+    from repsurf_amd import objectives
+    rows = 260
+    z = logits_of(rows, classes, dtype, seed=classes, pad=1 if classes % 2 else 0).requires_grad_(True)
+    y = targets_of(rows, classes, seed=classes, ignored=0.1)
+    counts = (y != IGN)
+    n = int(counts.sum())
+    x = z.detach().double()
+    lp = torch.log_softmax(x, 1)
+    want = torch.where(counts.cuda(), lp.gather(1, y.clamp_min(0).cuda()[:, None])[:, 0], 0.0)
+    bound = (3 * (lp.exp() * (x - x.amax(1, keepdim=True)).abs()).sum(1) + 6) * U
+    ratio = RATIOS[torch.randint(0, len(RATIOS), (rows,), generator=torch.Generator().manual_seed(1))].cuda()
+    old = (want - ratio.log()).float()
+    adv = torch.randn(rows, generator=torch.Generator().manual_seed(2)).cuda()
+    got = objectives.policy_loss(z, y.cuda(), old, adv)
+    assert ((got.logp.double() - want).abs() <= bound + U * want.abs()).all()
+    r, a = torch.exp(want - old.double()), adv.double()
+    each = torch.where(counts.cuda(), -torch.minimum(r * a, r.clamp(0.8, 1.2) * a), 0.0)
+    assert abs(float(got.loss.detach()) - float(each.sum() / n)) <= 1.01 * float((r * a.abs() * bound * counts.cuda()).sum() / n) + 2 * U * abs(float(each.sum() / n))
+    g, = torch.autograd.grad(got.loss, z)
+    assert (g[~counts.cuda()] == 0).all()
+    pick = [i for i in (0, 1, 2, 100, 255, 256, 258, 259) if counts[i]]
+    ref = Ref(z.detach()[pick], y[pick])
+    cut = torch.where(a >= 0, r > 1.2, r < 0.8)
+    c = torch.where(cut, 0.0, -a * r / n)[pick].cpu()
+    w, = torch.autograd.grad(ref.logp, ref.z, c)
+    ref.check_grad(g[pick], w, dtype, c, 1.01 * c.abs() * ref.L + U * c.abs())
+    alone = objectives.token_logprobs(z, y.cuda())
+    assert ((alone.detach().double() - want).abs() <= bound + U * want.abs()).all()
+    up = torch.randn(rows, generator=torch.Generator().manual_seed(3))
+    g, = torch.autograd.grad(alone, z, up.cuda())
+    ref = Ref(z.detach()[pick], y[pick])
+    w, = torch.autograd.grad(ref.logp, ref.z, up[pick].double())
+    ref.check_grad(g[pick], w, dtype, up[pick].double(), torch.zeros(len(pick), dtype=torch.float64))
+    assert (g[~counts.cuda()] == 0).all()
+
+
 def test_policy_advantages_per_sequence_and_unit_gradient():
     from repsurf_amd import head, objectives
     lengths = [40, 0, 17, 33]
