@@ -660,9 +660,12 @@ typedef struct rs_logits {
 #define RS_LOGITS_FEW_ROWS 256
 #define RS_LOGITS_PARTS 64
 int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64, float *stat, void *scratch, void *stream);
-/* dlogits (rows, classes; contiguous, of the logits' type) = c * ([j = target] - softmax_j), c = coef[row] -- with offsets coef[sequence] --
- * times *gout (NULL: 1).  skip_unit: nothing is done where *gout is 1 (dlogits holds that result already). */
-int rs_token_logprobs_backward(const rs_logits *l, const float *stat, const float *coef, const float *gout, int skip_unit, void *dlogits,
+/* dlogits (rows, classes; contiguous, of the logits' type) = c * ([j = target] - softmax_j), c = coef[row] -- with offsets coef[sequence],
+ * unless RS_BACKWARD_ROW_COEF says that every row has its own there too -- times *gout (NULL: 1).  Rows that do not count become zeros: none
+ * of their logits, stat and coef is read.  RS_BACKWARD_SKIP_UNIT: nothing is done where *gout is 1 (dlogits holds that result already). */
+#define RS_BACKWARD_SKIP_UNIT 1
+#define RS_BACKWARD_ROW_COEF 2
+int rs_token_logprobs_backward(const rs_logits *l, const float *stat, const float *coef, const float *gout, int flags, void *dlogits,
                                void *stream);
 /* per sequence: the sum of its rows' log-probabilities, or (average) their mean over the rows that count: sums (fp64), out (fp32), each
  * (fp32) = the factor of a row in it; any of the three may be NULL */
@@ -676,7 +679,7 @@ int rs_preference_pairs(int pairs, const double *sums, const float *each, const 
  *   -min(r A, clamp(r, low, high) A) + kl_coef (exp(d) - 1 - d),  d = ref_logp - x (ref_logp NULL: without that term)
  * averaged over the rows that count (token_mean), or over every sequence's rows and then over the sequences (one without any adds 0).
  * stats (2) = mean of exp(d) - 1 - d, share of rows whose ratio was cut off (both weighted like the loss).  With dlogits: the
- * gradient, and coef (rows) / stat (rows, 2) for rs_token_logprobs_backward. */
+ * gradient, and coef (rows) / stat (rows, 2) for rs_token_logprobs_backward (RS_BACKWARD_ROW_COEF where there are offsets). */
 typedef struct rs_policy {
   const float *old_logp, *advantages, *ref_logp;
   int advantages_per_sequence, token_mean;

@@ -207,9 +207,14 @@ struct Outs {                 // what a kernel writes of a row; null: not wanted
   double *logp64;
   float2 *stat;               // M, 1 / s
   void *dz;
-  const float *coef, *up;     // LG_BACK: coefficients of rows (of sequences with offsets), and a factor for all of them
-  int skip_unit;
+  const float *coef, *up;     // LG_BACK: coefficients of rows (of sequences with offsets, unless row_coef), and a factor for all of them
+  int skip_unit, row_coef;
 };
+
+// LG_BACK: a row's coefficient.  With offsets too where every row has its own: they tell which rows lie behind the last sequence.
+__device__ __forceinline__ float lg_coef(const Rows &R, const Outs &O, const Row &w) {
+  return O.coef[R.offset && !O.row_coef ? (long long)w.owner : w.at];
+}
 
 // one that does not count, or whose target is no class: 0, or not a number; none of its logits is read
 __device__ __forceinline__ float lg_void(const Rows &R, const Policy &P, const Outs &O, const Row &w, bool first, int policy, double *add) {
@@ -311,7 +316,7 @@ short_kernel(Rows R, Policy P, Outs O) {
 #pragma unroll
       for (int q = 0; q < SUB; ++q) {
         c[q] = 0.f; M[q] = 0.f; inv[q] = 0.f;
-        if (w[q].counts) c[q] = w[q].bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w[q].owner : w[q].at] * up;
+        if (w[q].counts) c[q] = w[q].bad ? __uint_as_float(0x7FC00000u) : lg_coef(R, O, w[q]) * up;
         if (in[q]) { const float2 st = O.stat[w[q].at]; M[q] = st.x; inv[q] = st.y; }
       }
     } else {
@@ -522,7 +527,7 @@ long_back_kernel(Rows R, Outs O, int parts) {
   for (long long row = blockIdx.y; row < R.rows; row += gridDim.y) {
     const Row w = lg_row(R, row);
     float c = 0.f;
-    if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : O.coef[R.offset ? (long long)w.owner : row] * up;
+    if (w.counts) c = w.bad ? __uint_as_float(0x7FC00000u) : lg_coef(R, O, w) * up;
     const T *__restrict__ z = (const T *)R.z + row * R.ld;
     T *__restrict__ dz = (T *)O.dz + row * V;
     if (c == 0.f || c != c) {
@@ -793,10 +798,8 @@ int run_rows(const rs_logits *l, const Policy &P, const Outs &O, void *scratch, 
     n = (int)l->rows;
     if (MODE == LG_POLICY && O.dz) {
       Outs B = O;
-      B.coef = P.coef; B.up = nullptr; B.skip_unit = 0;
-      Rows Q = R;
-      Q.offset = nullptr; Q.sequences = 0;                     // (coef is per row, 0 for those behind the last sequence)
-      LG_TYPE(l->type, (launch_rows<T, LG_BACK>(l, Q, P, B, st)));
+      B.coef = P.coef; B.row_coef = 1;
+      LG_TYPE(l->type, (launch_rows<T, LG_BACK>(l, R, P, B, st)));
     }
   } else {
     LG_TYPE(l->type, n = (launch_rows<T, MODE>(l, R, P, O, st)));
@@ -811,18 +814,19 @@ extern "C" int rs_token_logprobs(const rs_logits *l, float *logp, double *logp64
   if (rc != RS_OK) return rc;
   if (l->rows == 0) return RS_OK;
   RS_REQUIRE(logp || logp64, "rs_token_logprobs: null pointer");
-  run_rows<LG_LOGP>(l, Policy{}, Outs{logp, logp64, (float2 *)stat, nullptr, nullptr, nullptr, 0}, scratch, (hipStream_t)stream);
+  run_rows<LG_LOGP>(l, Policy{}, Outs{logp, logp64, (float2 *)stat, nullptr, nullptr, nullptr, 0, 0}, scratch, (hipStream_t)stream);
   RS_CHECK_LAUNCH("rs_token_logprobs");
   return RS_OK;
 }
 
-extern "C" int rs_token_logprobs_backward(const rs_logits *l, const float *stat, const float *coef, const float *gout, int skip_unit, void *dlogits,
+extern "C" int rs_token_logprobs_backward(const rs_logits *l, const float *stat, const float *coef, const float *gout, int flags, void *dlogits,
                                           void *stream) {
   const int rc = check_rows(l, "rs_token_logprobs_backward");
   if (rc != RS_OK) return rc;
   if (l->rows == 0) return RS_OK;
   RS_REQUIRE(stat && coef && dlogits, "rs_token_logprobs_backward: null pointer");
-  const Outs O{nullptr, nullptr, (float2 *)stat, dlogits, coef, gout, skip_unit};
+  RS_REQUIRE(!(flags & ~(RS_BACKWARD_SKIP_UNIT | RS_BACKWARD_ROW_COEF)), "rs_token_logprobs_backward: flags=%d", flags);
+  const Outs O{nullptr, nullptr, (float2 *)stat, dlogits, coef, gout, flags & RS_BACKWARD_SKIP_UNIT, flags & RS_BACKWARD_ROW_COEF};
   LG_TYPE(l->type, (launch_rows<T, LG_BACK>(l, rows_of(l), Policy{}, O, (hipStream_t)stream)));
   RS_CHECK_LAUNCH("rs_token_logprobs_backward");
   return RS_OK;
@@ -869,7 +873,7 @@ extern "C" int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stre
   if (l->rows > 0) {
     const Policy P{p->old_logp, p->advantages, p->ref_logp, p->advantages_per_sequence, p->token_mean, p->low, p->high, p->kl_coef, p->counts, (int)splits,
                    p->coef, p->partial};
-    n = run_rows<LG_POLICY>(l, P, Outs{p->logp, nullptr, (float2 *)p->stat, p->dlogits, nullptr, nullptr, 0}, p->scratch, st);
+    n = run_rows<LG_POLICY>(l, P, Outs{p->logp, nullptr, (float2 *)p->stat, p->dlogits, nullptr, nullptr, 0, 0}, p->scratch, st);
   }
   hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, n, p->partial, p->loss, p->stats);
   RS_CHECK_LAUNCH("rs_policy_loss");

@@ -26,6 +26,7 @@ P, c_int, c_ll, c_double = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, cty
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POLICY_COUNTS, POLICY_GROUPS = 64, 8192          # RS_POLICY_COUNTS, RS_POLICY_GROUPS
 FEW_ROWS, PARTS = 256, 64                         # RS_LOGITS_FEW_ROWS, RS_LOGITS_PARTS
+SKIP_UNIT, ROW_COEF = 1, 2                        # RS_BACKWARD_SKIP_UNIT, RS_BACKWARD_ROW_COEF
 
 PolicyLoss = namedtuple("PolicyLoss", "loss logp kl clip_fraction")
 PreferenceLoss = namedtuple("PreferenceLoss", "loss chosen_rewards rejected_rewards")
@@ -102,7 +103,7 @@ def _call(device, name, *args):
             _lib.call(name, *args, _lib.current_stream())
 
 
-def _backward(ctx, logits, target, offset, work, coef, gout, skip_unit=0, out=None):
+def _backward(ctx, logits, target, offset, work, coef, gout, flags=0, out=None):
     """from the tensors as autograd hands them back (a hook may have moved them); the rows' stat lies in `work`, ctx.stat floats from its
     start; coef: an address.  (Autograd runs this on a thread of its own, whose every line costs twice what it costs elsewhere.)"""
     if out is None:
@@ -114,7 +115,7 @@ def _backward(ctx, logits, target, offset, work, coef, gout, skip_unit=0, out=No
             desc.offset = offset.data_ptr()
     if gout is not None:
         gout = (gout if gout.dtype is torch.float32 else gout.to(torch.float32)).data_ptr()
-    _call(logits.device, "rs_token_logprobs_backward", ctx.ref, work.data_ptr() + 4 * ctx.stat, coef, gout, skip_unit, out.data_ptr())
+    _call(logits.device, "rs_token_logprobs_backward", ctx.ref, work.data_ptr() + 4 * ctx.stat, coef, gout, flags, out.data_ptr())
     return out
 
 
@@ -280,8 +281,7 @@ class _Policy(Function):
                        coef if held else None, stat if held else None, scratch if room else None)
         _call(logits.device, "rs_policy_loss", ctypes.byref(desc), ctypes.byref(p))
         if grad:
-            desc.offset, desc.sequences = None, 0           # (coef is per row, 0 for the rows behind the last sequence)
-            _keep(ctx, desc, (stat - at) // 4, logits, target, work)
+            _keep(ctx, desc, (stat - at) // 4, logits, target, work, offset)
             ctx.d = d
         ctx.mark_non_differentiable(logp, stats)
         return loss, logp, stats
@@ -289,7 +289,7 @@ class _Policy(Function):
     @staticmethod
     @_once
     def backward(ctx, g, *_):
-        logits, target, work = ctx.saved_tensors
+        logits, target, work, offset = ctx.saved_tensors
         d = ctx.d
         first = d is not None
         ctx.d = None                       # handed out once: a second pass over a retained graph computes it again
@@ -298,7 +298,7 @@ class _Policy(Function):
             if one is not None and g.data_ptr() == one.data_ptr():          # loss.backward(unit_gradient(device))
                 return (d,) + (None,) * 11
         coef = work.data_ptr() + 4 * (ctx.stat + 2 * logits.shape[0])
-        return (_backward(ctx, logits, target, None, work, coef, g, int(first), d),) + (None,) * 11
+        return (_backward(ctx, logits, target, offset, work, coef, g, ROW_COEF | (SKIP_UNIT if first else 0), d),) + (None,) * 11
 
 
 def policy_loss(logits, target, old_logp, advantages, ref_logp=None, offset=None, clip=(0.2, 0.2), kl_coef=0.0, reduction="token", ignore_index=-100):

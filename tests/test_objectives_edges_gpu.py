@@ -1,0 +1,55 @@
+"""repsurf_amd.objectives where a call meets something unusual."""
+import math
+
+import pytest
+import torch
+
+from tests.test_objectives_gpu import ends, logits_of, targets_of
+
+pytestmark = pytest.mark.gpu
+
+
+def bits(t):
+    return t.view(torch.int32 if t.element_size() == 4 else torch.int16)
+
+
+# ---- rows behind the last sequence ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("classes", [13, 1500, 20001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [[40, 17], [200, 0, 100]])          # (57 rows of 20001 classes are cut over many workgroups, 300 are not)
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_rows_behind_the_last_sequence_may_hold_anything(classes, dtype, lengths, reduction):
+    """The same bits as with well-behaved padding, whatever the upstream gradient is and however often it is asked for; and zeros there."""
+    from repsurf_amd import head, objectives
+    n, behind = sum(lengths), 6
+    z = logits_of(n + behind, classes, dtype, seed=classes)
+    y = targets_of(n + behind, classes, seed=1, ignored=0.1)
+    off = ends(lengths)
+    g = torch.Generator().manual_seed(3)
+    old, adv = (torch.randn(n + behind, generator=g) - math.log(classes)).cuda(), torch.randn(n + behind, generator=g).cuda()
+    y[n:] = torch.arange(behind) % classes
+    odd, yo, oo, ao = z.clone(), y.clone(), old.clone(), adv.clone()
+    odd[n] = float("nan"); odd[n + 1, 1] = float("inf"); odd[n + 2] = 100.0; odd[n + 3] = torch.finfo(dtype).max; odd[n + 4, :] = -math.inf
+    yo[n + 4], yo[n + 5] = -7, classes
+    oo[n:], ao[n:] = float("nan"), float("inf")
+    before = head.bad_label_count(z.device)
+
+    def run(zz, yy, old_, adv_):
+        zz = zz.detach().clone().requires_grad_(True)
+        out = objectives.policy_loss(zz, yy.cuda(), old_, adv_, offset=off, reduction=reduction)
+        grads = [torch.autograd.grad(out.loss, zz, retain_graph=True)[0] for _ in range(2)]          # handed out, then computed again
+        grads.append(torch.autograd.grad(out.loss * 0.3, zz)[0])
+        fresh = objectives.policy_loss(zz, yy.cuda(), old_, adv_, offset=off, reduction=reduction)
+        grads.append(torch.autograd.grad(fresh.loss * 0.3, zz)[0])
+        grads.append(torch.autograd.grad(objectives.sequence_logprobs(zz, yy.cuda(), off).sum(), zz)[0])
+        if len(lengths) % 2 == 0:
+            grads.append(torch.autograd.grad(objectives.preference_loss(zz, yy.cuda(), off, torch.zeros(len(lengths), device="cuda")).loss, zz)[0])
+        return out, grads
+
+    want, clean = run(z, y, old, adv)
+    got, grads = run(odd, yo, oo, ao)
+    assert head.bad_label_count(z.device) == before
+    assert torch.isfinite(want.loss) and torch.equal(want.loss, got.loss) and torch.equal(want.logp, got.logp)
+    for i, (a, b) in enumerate(zip(clean, grads)):
+        assert (b[n:] == 0).all(), i
+        assert torch.equal(bits(a[:n]), bits(b[:n])), i
