@@ -302,7 +302,7 @@ class AdamW(Adam):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes its own state dicts and torch.optim.AdamW's; fp32 moments are rounded to 8 bits (to nearest) where state_bits is 8, and
-        8-bit ones are refused where it is 32.  The values are copied."""
+        8-bit ones are refused where it is 32.  The values are copied; a parameter without any starts anew."""
         bits = {32 if v["exp_avg"].is_floating_point() else 8 for v in state_dict["state"].values() if "exp_avg" in v}
         if len(bits) > 1 or (bits == {8} and self.state_bits == 32):
             raise ValueError("AdamW.load_state_dict: 8-bit moments need state_bits=8 (and all of them)")
@@ -317,9 +317,13 @@ class AdamW(Adam):
                 for name, v in saved.items():
                     if name in ("exp_avg", "exp_avg_sq", "low") and tuple(v.shape) != tuple(p.shape):
                         raise ValueError(f"AdamW.load_state_dict: {name} of parameter {k} has shape {tuple(v.shape)}, the parameter {tuple(p.shape)}")
+        # state_dict() hands out views of the buffers that are written below: such values are read whole before anything is
+        own = {buf.untyped_storage().data_ptr() for st in self._dev.values() for buf in st["flat"].values()}
+        kept = lambda v: v.clone() if torch.is_tensor(v) and v.untyped_storage().data_ptr() in own else v      # noqa: E731
+        state = {k: {name: kept(v) for name, v in s.items()} for k, s in state_dict["state"].items()}
         super(Adam, self).load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for gi, (keys, group) in enumerate(zip(order, self.param_groups)):
-            saved = [state_dict["state"].get(k, {}) for k in keys]
+            saved = [state.get(k, {}) for k in keys]
             if gi not in self._dev and not any("exp_avg" in s for s in saved):
                 continue
             dev = group["params"][0].device
