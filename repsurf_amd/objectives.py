@@ -119,10 +119,13 @@ def _backward(ctx, logits, target, offset, work, coef, gout, flags=0, out=None):
     return out
 
 
-def _once(fn):
-    """a backward pass that can be differentiated no further; the wrapper that says so is entered only where somebody builds its graph"""
-    careful = once_differentiable(fn)
-    return lambda ctx, *g: careful(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
+def _once(inputs):
+    """a backward pass over so many inputs that can be differentiated no further; the wrapper that says so is entered only where somebody
+    builds its graph.  Where nothing came down to the first output (the only one that is differentiable) there is no gradient."""
+    def wrap(fn):
+        careful, none = once_differentiable(fn), (None,) * inputs
+        return lambda ctx, g, *rest: none if g is None else careful(ctx, g, *rest) if torch.is_grad_enabled() else fn(ctx, g, *rest)
+    return wrap
 
 
 def _keep(ctx, desc, stat, *tensors):
@@ -167,7 +170,7 @@ class _TokenLogprobs(Function):
         return logp
 
     @staticmethod
-    @_once
+    @_once(4)
     def backward(ctx, g):
         logits, target, work = ctx.saved_tensors
         g = _as(g, torch.float32)
@@ -207,7 +210,7 @@ class _SequenceLogprobs(Function):
         return out
 
     @staticmethod
-    @_once
+    @_once(6)
     def backward(ctx, g):
         logits, target, offset, buf = ctx.saved_tensors
         coef = _as(g, torch.float32) * buf[buf.numel() - offset.numel():]
@@ -236,7 +239,7 @@ class _Preference(Function):
         return loss, rewards
 
     @staticmethod
-    @_once
+    @_once(9)
     def backward(ctx, g, _):
         logits, target, offset, buf = ctx.saved_tensors
         return (_backward(ctx, logits, target, offset, buf, buf.data_ptr() + 4 * ctx.coef, g),) + (None,) * 8
@@ -287,7 +290,7 @@ class _Policy(Function):
         return loss, logp, stats
 
     @staticmethod
-    @_once
+    @_once(12)
     def backward(ctx, g, *_):
         logits, target, work, offset = ctx.saved_tensors
         d = ctx.d

@@ -1,0 +1,56 @@
+"""repsurf_amd.objectives without a device, where a call meets something unusual: its autograd code with a recorder in the kernels' place."""
+import pytest
+import torch
+
+from repsurf_amd import objectives as O
+
+ROWS, CLASSES = 6, 5
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """the ABI calls that would be made: (name, arguments); descriptors as dicts of what stood in them"""
+    made = []
+
+    def record(device, name, *args):
+        made.append((name, [{f: getattr(a._obj, f) for f, _ in a._obj._fields_} if hasattr(a, "_obj") else a for a in args]))
+
+    monkeypatch.setattr(O, "_call", record)
+    monkeypatch.setitem(O._bad, None, 0)
+    return made
+
+
+def leaf():
+    return torch.randn(ROWS, CLASSES, generator=torch.Generator().manual_seed(0)).requires_grad_(True)
+
+
+def functions(z):
+    y, off, one = torch.zeros(ROWS, dtype=torch.long), torch.tensor([2, 5], dtype=torch.int32), torch.ones(ROWS)
+    return {"token": lambda: O._TokenLogprobs.apply(z, y, -100, True), "sequence": lambda: O._SequenceLogprobs.apply(z, y, off, -100, False, True),
+            "preference": lambda: O._Preference.apply(z, y, off, torch.zeros(2), 0.1, 0.0, False, -100, True)[0],
+            "policy": lambda: O._Policy.apply(z, y, one, one, None, off, 0.8, 1.2, 0.0, True, -100, True)[0]}
+
+
+NAMES = ["token", "sequence", "preference", "policy"]
+
+
+class Drop(torch.autograd.Function):
+    """hands nothing on: its input has no gradient"""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_no_upstream_gradient_is_no_gradient(calls, name):
+    z = leaf()
+    out = functions(z)[name]()
+    assert torch.autograd.grad(Drop.apply(out).sum(), z, allow_unused=True) == (None,)
+    assert not any(n.endswith("backward") for n, _ in calls)
+    torch.autograd.grad(functions(z)[name]().sum(), z)
+    assert sum(n.endswith("backward") for n, _ in calls) == 1

@@ -53,3 +53,44 @@ def test_rows_behind_the_last_sequence_may_hold_anything(classes, dtype, lengths
     for i, (a, b) in enumerate(zip(clean, grads)):
         assert (b[n:] == 0).all(), i
         assert torch.equal(bits(a[:n]), bits(b[:n])), i
+
+
+# ---- an upstream gradient that does not exist -------------------------------------------------------------------------
+class Drop(torch.autograd.Function):
+    """hands nothing on: its input has no gradient"""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def small_case(classes=13, seed=7):
+    z = logits_of(50, classes, torch.float32, seed=seed)
+    y = targets_of(50, classes, seed=seed).cuda()
+    g = torch.Generator().manual_seed(seed)
+    return z, y, ends([30, 20]), (torch.randn(50, generator=g) - 2).cuda(), torch.randn(50, generator=g).cuda(), torch.tensor([-60.0, -50.0]).cuda()
+
+
+def losses(z, y, off, old, adv, pref):
+    from repsurf_amd import objectives
+    return {"token": lambda: objectives.token_logprobs(z, y), "sequence": lambda: objectives.sequence_logprobs(z, y, off, average=True),
+            "preference": lambda: objectives.preference_loss(z, y, off, pref).loss, "policy": lambda: objectives.policy_loss(z, y, old, adv, offset=off).loss}
+
+
+@pytest.mark.parametrize("name", ["token", "sequence", "preference", "policy"])
+@pytest.mark.parametrize("unit", [False, True])
+def test_no_upstream_gradient_is_no_gradient(name, unit):
+    from repsurf_amd import head
+    z, *rest = small_case()
+    z.requires_grad_(True)
+    if unit:
+        head.unit_gradient(z.device)
+    f = losses(z, *rest)[name]
+    assert torch.autograd.grad(Drop.apply(f()).sum(), z, allow_unused=True) == (None,)
+    w = torch.randn(z.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    g, = torch.autograd.grad(Drop.apply(f()).sum() + (z * w).sum(), z)
+    assert torch.equal(g, w)
