@@ -66,7 +66,7 @@ def _logits(logits, target, offset):
 def _as(t, dtype):
     """data (not differentiated) as a dense tensor of a type"""
     if t.dtype is dtype and t.is_contiguous():
-        return t
+        return t.detach() if t.requires_grad else t
     return t.detach().to(dtype).contiguous()
 
 

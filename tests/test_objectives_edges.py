@@ -54,3 +54,13 @@ def test_no_upstream_gradient_is_no_gradient(calls, name):
     assert not any(n.endswith("backward") for n, _ in calls)
     torch.autograd.grad(functions(z)[name]().sum(), z)
     assert sum(n.endswith("backward") for n, _ in calls) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_data_is_taken_out_of_its_graph(dtype):
+    t = torch.ones(ROWS, dtype=dtype, requires_grad=True)
+    for data in (t, t * 2, t[::1], t.detach()):
+        got = O._values("data", data, (ROWS,), leaf())
+        assert got.dtype is torch.float32 and not got.requires_grad and torch.equal(got, data.detach().float())
+    plain = torch.ones(ROWS)
+    assert O._values("data", plain, (ROWS,), leaf()) is plain

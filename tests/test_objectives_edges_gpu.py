@@ -94,3 +94,27 @@ def test_no_upstream_gradient_is_no_gradient(name, unit):
     w = torch.randn(z.shape, generator=torch.Generator().manual_seed(1)).cuda()
     g, = torch.autograd.grad(Drop.apply(f()).sum() + (z * w).sum(), z)
     assert torch.equal(g, w)
+
+
+# ---- data that would have a gradient --------------------------------------------------------------------------------
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_data_has_no_gradient(frozen, dtype):
+    """scores of another network taken outside no_grad, advantages of a value head: the same bits as detached, and no gradient for them"""
+    from repsurf_amd import objectives
+    z, y, off, old, adv, pref = small_case()
+    z.requires_grad_(not frozen)
+    other = logits_of(50, 13, torch.float32, seed=9).requires_grad_(True)
+    score, sums = objectives.token_logprobs(other, y).to(dtype), objectives.sequence_logprobs(other, y, off).to(dtype)
+    value = adv.to(dtype).requires_grad_(True)
+
+    def policy(o, a, r):
+        return objectives.policy_loss(z, y, o, a, ref_logp=r, offset=off, kl_coef=0.1)
+
+    for got, want in ((policy(score, value, score), policy(score.detach(), value.detach(), score.detach())),
+                      (objectives.preference_loss(z, y, off, sums), objectives.preference_loss(z, y, off, sums.detach()))):
+        assert torch.equal(got.loss, want.loss) and got.loss.requires_grad != frozen
+        if not frozen:
+            a, b, c = torch.autograd.grad(got.loss, (z, other, value), allow_unused=True)
+            d, = torch.autograd.grad(want.loss, z)
+            assert torch.equal(a, d) and b is None and c is None
