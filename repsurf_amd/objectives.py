@@ -12,12 +12,13 @@ outside [0, classes) makes its row NaN and is counted by head.bad_label_count, a
     policy_loss          clipped policy objective with a KL term against a reference policy
 
 A row's statistics are collected in fp64; gradients are rounded once, to the logits' type.  The losses are differentiable in `logits` alone
-(once); the other tensors are data.  The calls allocate through torch and can be captured into a graph once they ran eagerly."""
+(once, by backward passes; forward-mode tangents are refused); the other tensors are data.  The calls allocate through torch and can be
+captured into a graph once they ran eagerly."""
 import ctypes
 from collections import namedtuple
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, head
@@ -43,8 +44,15 @@ class PolicyDesc(ctypes.Structure):          # rs_policy
                 ("loss", P), ("stats", P), ("logp", P), ("dlogits", P), ("coef", P), ("stat", P), ("scratch", P)]
 
 
+def _no_tangent(t):
+    """forward-mode derivatives are refused: nothing here would carry a tangent on"""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:      # (below 0: no level is entered)
+        raise NotImplementedError("objectives: forward-mode derivatives are not offered")
+
+
 def _logits(logits, target, offset):
     """checks, and the tensors as the kernels take them"""
+    _no_tangent(logits)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"objectives: logits must be (rows, classes), got {tuple(logits.shape)}")
     if logits.dtype not in _TYPES:
@@ -71,6 +79,7 @@ def _as(t, dtype):
 
 
 def _values(name, t, shape, logits):
+    _no_tangent(t)
     if t.shape != shape:
         raise ValueError(f"objectives: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != logits.device:

@@ -64,3 +64,18 @@ def test_data_is_taken_out_of_its_graph(dtype):
         assert got.dtype is torch.float32 and not got.requires_grad and torch.equal(got, data.detach().float())
     plain = torch.ones(ROWS)
     assert O._values("data", plain, (ROWS,), leaf()) is plain
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    y, off, one, two = torch.zeros(ROWS, dtype=torch.long), torch.tensor([2, 5], dtype=torch.int32), torch.ones(ROWS), torch.zeros(2)
+    with fw.dual_level():
+        for z in (leaf().detach(), leaf()):
+            dual = fw.make_dual(z, torch.ones_like(z))
+            for call in (lambda: O.token_logprobs(dual, y), lambda: O.sequence_logprobs(dual, y, off), lambda: O.preference_loss(dual, y, off, two),
+                         lambda: O.policy_loss(dual, y, one, one)):
+                with pytest.raises(NotImplementedError):
+                    call()
+        with pytest.raises(NotImplementedError):
+            O._values("data", fw.make_dual(one, one), (ROWS,), leaf())
+        assert O._values("data", one, (ROWS,), leaf()) is one

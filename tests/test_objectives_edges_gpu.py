@@ -118,3 +118,25 @@ def test_data_has_no_gradient(frozen, dtype):
             a, b, c = torch.autograd.grad(got.loss, (z, other, value), allow_unused=True)
             d, = torch.autograd.grad(want.loss, z)
             assert torch.equal(a, d) and b is None and c is None
+
+
+# ---- forward-mode derivatives are not offered ---------------------------------------------------------------------------
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    from repsurf_amd import objectives
+    z, y, off, old, adv, pref = small_case()
+    calls = [lambda t: objectives.token_logprobs(t, y), lambda t: objectives.sequence_logprobs(t, y, off), lambda t: objectives.preference_loss(t, y, off, pref),
+             lambda t: objectives.policy_loss(t, y, old, adv)]
+    data = [lambda t: objectives.preference_loss(z, y, off, t(pref)), lambda t: objectives.policy_loss(z, y, t(old), adv),
+            lambda t: objectives.policy_loss(z, y, old, t(adv)), lambda t: objectives.policy_loss(z, y, old, adv, ref_logp=t(old), kl_coef=0.1)]
+    want = [f(z) for f in calls[:2]]
+    with fw.dual_level():
+        for f in calls:
+            for leaf in (z, z.clone().requires_grad_(True)):
+                with pytest.raises(NotImplementedError):
+                    f(fw.make_dual(leaf, torch.ones_like(leaf)))
+        for f in data:
+            with pytest.raises(NotImplementedError):
+                f(lambda t: fw.make_dual(t, torch.ones_like(t)))
+        assert all(torch.equal(f(z), w) for f, w in zip(calls, want))          # no tangent: nothing to refuse
+    assert all(torch.equal(f(z), w) for f, w in zip(calls, want))
