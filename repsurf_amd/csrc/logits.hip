@@ -157,8 +157,14 @@ __device__ __forceinline__ double lg_log64(double s) {                  // of a 
   const double q = fma(s, lg_exp64(-y), -1.0);
   return s < INFINITY ? y + fma(-0.5 * q, q, q) : s;
 }
-__device__ __forceinline__ double lg_rest(double d) {                    // exp(d) - 1 - d
-  return fabs(d) <= 0.35 ? d * d * lg_taylor(d, 0.5) : lg_exp64(d) - 1.0 - d;
+__device__ __forceinline__ double lg_rest(double d, double *slope) {     // exp(d) - 1 - d, and its slope exp(d) - 1 (each by itself: d may be -infinity)
+  if (fabs(d) <= 0.35) {
+    const double e = d * d * lg_taylor(d, 0.5);
+    *slope = e + d;
+    return e;
+  }
+  *slope = lg_exp64(d) - 1.0;
+  return *slope - d;
 }
 
 // d loss / d log p(y) of the policy loss for one row, and its three contributions
@@ -168,9 +174,10 @@ __device__ __forceinline__ double lg_policy(const Policy &P, double w, double lo
   double each = -(cut ? (a >= 0.0 ? P.hi : P.lo) : r) * a, c = cut ? 0.0 : -a * r;
   if (r != r || a != a) each = c = r + a;
   if (P.ref) {
-    const double d = ref - logp, e = lg_rest(d);               // not negative, and its mean over the policy's own draws is the KL
+    double slope;
+    const double e = lg_rest(ref - logp, &slope);              // not negative, and its mean over the policy's own draws is the KL
     each += P.kl * e;
-    c -= P.kl * (e + d);
+    c -= P.kl * slope;
     add[1] += w * e;
   }
   add[0] += w * each;

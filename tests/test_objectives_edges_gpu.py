@@ -140,3 +140,31 @@ def test_forward_mode_is_refused():
                 f(lambda t: fw.make_dual(t, torch.ones_like(t)))
         assert all(torch.equal(f(z), w) for f, w in zip(calls, want))          # no tangent: nothing to refuse
     assert all(torch.equal(f(z), w) for f, w in zip(calls, want))
+
+
+# ---- a reference that masks the taken class -----------------------------------------------------------------------------
+@pytest.mark.parametrize("classes", [13, 1500, 20001])
+@pytest.mark.parametrize("rows", [24, 300])
+def test_a_reference_that_masks_the_taken_class(classes, rows):
+    """exp(d) - 1 - d is infinite there, its slope exp(d) - 1 is -1; the rows beside it keep theirs.  Tolerances as in the policy tests: of a
+    coefficient what the log-probability moves it by, and its rounding."""
+    from repsurf_amd import objectives
+    from tests.test_objectives_gpu import U, Ref
+    z, y = logits_of(rows, classes, torch.float32, seed=4).requires_grad_(True), targets_of(rows, classes, seed=4)
+    y[2], y[5] = 1, 2
+    ref = Ref(z, y)
+    g = torch.Generator().manual_seed(6)
+    x = ref.logp.detach()
+    old, adv, other = (x - 0.05).float(), torch.randn(rows, generator=g), (x + torch.randn(rows, generator=g)).float()
+    other[2], other[5], kl = -math.inf, -1e30, 0.05
+    out = objectives.policy_loss(z, y.cuda(), old.cuda(), adv.cuda(), ref_logp=other.cuda(), kl_coef=kl)
+    assert float(out.loss) == math.inf and float(out.kl) == math.inf
+    w = ref.counts / int(ref.counts.sum())
+    r, d, a = torch.exp(x - old.double()), other.double() - x, adv.double()
+    c = w * (-a * r - kl * torch.expm1(d))
+    sens = w * (r * a.abs() + kl * torch.exp(d))
+    want, = torch.autograd.grad(ref.logp, ref.z, c, retain_graph=True)
+    for factor in (1.0, 0.5):
+        got, = torch.autograd.grad(out.loss * factor, z, retain_graph=True)
+        assert torch.isfinite(got).all()
+        ref.check_grad(got, want * factor, torch.float32, c * factor, factor * (1.01 * sens * ref.L + 3 * U * c.abs()))
