@@ -694,9 +694,10 @@ pairs_kernel(int pairs, const double *__restrict__ sums, const float *__restrict
   double t = 0.0;
   for (int i = threadIdx.x; i < pairs; i += 256) {
     const double a = beta * (sums[i] - (double)ref[i]), b = beta * (sums[pairs + i] - (double)ref[pairs + i]), h = a - b;
-    const double tail = log1p(exp(-fabs(h)));                  // -log sigmoid(+-h) = tail + max(-+h, 0)
+    const double e = exp(-fabs(h)), tail = log1p(e);           // -log sigmoid(+-h) = tail + max(-+h, 0)
     t += (1.0 - smooth) * (tail + fmax(-h, 0.0)) + (smooth > 0.0 ? smooth * (tail + fmax(h, 0.0)) : 0.0);   // (h may be infinite)
-    const double slope = (1.0 / (1.0 + exp(-h)) - (1.0 - smooth)) * beta / pairs;
+    // smooth - sigmoid(-h), from the exponential that does not overflow: sigmoid(h) - 1 would lose what is left of a pair far apart
+    const double slope = (smooth - (h >= 0.0 ? e : 1.0) / (1.0 + e)) * beta / pairs;
     rewards[i] = (float)a;
     rewards[pairs + i] = (float)b;
     coef[i] = (float)(slope * each[i]);

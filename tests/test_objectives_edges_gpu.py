@@ -168,3 +168,39 @@ def test_a_reference_that_masks_the_taken_class(classes, rows):
         got, = torch.autograd.grad(out.loss * factor, z, retain_graph=True)
         assert torch.isfinite(got).all()
         ref.check_grad(got, want * factor, torch.float32, c * factor, factor * (1.01 * sens * ref.L + 3 * U * c.abs()))
+
+
+# ---- pairs that are far apart -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+@pytest.mark.parametrize("apart", [0.0, 4.0, 30.0, 50.0, 80.0, -30.0, -50.0, -80.0])
+def test_the_slope_of_pairs_that_are_far_apart(apart, smoothing):
+    """h = `apart` and its neighbours.  d loss / dh = smoothing - sigmoid(-h); sigmoid(-h) moves by at most itself times dh, so what the sums
+    are off (beta L) is what it is off relatively; the coefficient adds the roundings of itself and of its two factors."""
+    from repsurf_amd import objectives
+    from tests.test_objectives_gpu import U, Ref
+    lengths, beta = [30, 11, 7, 19], 0.1
+    n = sum(lengths)
+    z, y = logits_of(n, 13, torch.float32, seed=8).requires_grad_(True), targets_of(n, 13, seed=8)
+    ref = Ref(z, y)
+    sums = torch.stack([p.sum() for p in ref.logp.split(lengths)])
+    other = sums.detach().clone()
+    other[0] -= apart / beta
+    other[1] -= (apart + 0.7) / beta
+    other = other.float()
+    r = beta * (sums - other.double())
+    h = r[:2] - r[2:]
+    ls = torch.nn.functional.logsigmoid
+    want = -((1 - smoothing) * ls(h) + smoothing * ls(-h)).mean()
+    got = objectives.preference_loss(z, y.cuda(), ends(lengths), other.cuda(), beta=beta, label_smoothing=smoothing)
+    dr = beta * torch.stack([x.sum() for x in (ref.L * ref.counts).split(lengths)])
+    dh = dr[:2] + dr[2:]
+    low = torch.sigmoid(-h.detach())
+    slope = smoothing - low                                    # d loss / dh, and what it may be off
+    off = low * torch.expm1(dh) + 2.0 ** -50 * (smoothing + low)
+    assert abs(float(got.loss) - float(want)) <= float(dh.mean()) + 2 * U * abs(float(want))
+    g, = torch.autograd.grad(got.loss, z)
+    spread = lambda t: torch.cat([t[i].expand(m) for i, m in enumerate(lengths)])      # noqa: E731
+    c = spread(torch.cat([slope, -slope]) * beta / 2)
+    w, = torch.autograd.grad(ref.logp, ref.z, c)
+    ref.check_grad(g, w, torch.float32, c, spread(torch.cat([off, off]) * beta / 2) + 4 * U * c.abs())
+    assert (g != 0).any()
