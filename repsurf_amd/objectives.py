@@ -66,9 +66,16 @@ def _logits(logits, target, offset):
         raise ValueError("objectives: all tensors must be on the logits' device")
     if device.type != "cuda":
         raise _lib.RepSurfHipError("repsurf_amd.objectives run on the HIP device only (got a CPU tensor); there is no CPU fallback")
-    if not logits.is_contiguous() and (logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]):
-        logits = logits.contiguous()
-    return logits, _as(target, torch.int64), None if offset is None else _as(offset, torch.int32)
+    return _pitched(logits)[0], _as(target, torch.int64), None if offset is None else _as(offset, torch.int32)
+
+
+def _pitched(logits):
+    """logits as the kernels take them (rows that lie dense, in order and apart), and the elements from one row to the next"""
+    classes = logits.shape[1]
+    if logits.is_contiguous():
+        return logits, classes
+    ld = logits.stride(0)
+    return (logits, ld) if logits.stride(1) == 1 and ld >= classes else (logits.contiguous(), classes)
 
 
 def _as(t, dtype):
@@ -113,15 +120,18 @@ def _call(device, name, *args):
 
 
 def _backward(ctx, logits, target, offset, work, coef, gout, flags=0, out=None):
-    """from the tensors as autograd hands them back (a hook may have moved them); the rows' stat lies in `work`, ctx.stat floats from its
-    start; coef: an address.  (Autograd runs this on a thread of its own, whose every line costs twice what it costs elsewhere.)"""
+    """from the tensors as autograd hands them back (a hook may have moved them, to another pitch too); the rows' stat lies in `work`, ctx.stat
+    floats from its start; coef: an address in it, or of a tensor that the caller holds.  (Autograd runs this on a thread of its own, whose every
+    line costs twice what it costs elsewhere.)"""
+    desc = ctx.desc
+    if (*logits.shape, _TYPES.get(logits.dtype)) != (desc.rows, desc.classes, desc.type):
+        raise _lib.RepSurfHipError("objectives: the saved logits came back with another shape or type")
     if out is None:
-        out = torch.empty_like(logits)          # (contiguous also where the logits have a pitch)
-    desc, at = ctx.desc, logits.data_ptr()
-    if at != desc.logits or target.data_ptr() != desc.target or (offset is not None and offset.data_ptr() != desc.offset):
-        desc.logits, desc.ld, desc.target = at, max(logits.stride(0), logits.shape[1]), target.data_ptr()
-        if offset is not None:
-            desc.offset = offset.data_ptr()
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)          # (also where the logits have a pitch)
+    logits, desc.ld = _pitched(logits)
+    desc.logits, desc.target = logits.data_ptr(), target.data_ptr()
+    if offset is not None:
+        desc.offset = offset.data_ptr()
     if gout is not None:
         gout = (gout if gout.dtype is torch.float32 else gout.to(torch.float32)).data_ptr()
     _call(logits.device, "rs_token_logprobs_backward", ctx.ref, work.data_ptr() + 4 * ctx.stat, coef, gout, flags, out.data_ptr())
@@ -285,7 +295,7 @@ class _Policy(Function):
         count_at = scratch + 4 * room
         stat = count_at + 4 * counts
         coef = stat + 8 * rows
-        d = torch.empty_like(logits) if grad else None
+        d = torch.empty_like(logits, memory_format=torch.contiguous_format) if grad else None
         held = grad and rows > 0
         desc = _desc(logits, target, ignore_index, offset)
         p = PolicyDesc(old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr(), int(adv.dim() == 2), int(token_mean), low, high, kl_coef,

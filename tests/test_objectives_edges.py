@@ -79,3 +79,52 @@ def test_forward_mode_is_refused():
         with pytest.raises(NotImplementedError):
             O._values("data", fw.make_dual(one, one), (ROWS,), leaf())
         assert O._values("data", one, (ROWS,), leaf()) is one
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("kind", ["dense", "columns", "pitched"])
+def test_saved_logits_that_come_back_in_another_layout(calls, name, kind):
+    """a hook that packs pitched logits and unpacks them at the very address where they lay, dense (as a freed buffer is handed out again):
+    what the backward pass is told about them is what came back"""
+    room = torch.zeros(ROWS * 16)
+    z = room.view(ROWS, 16)[:, :CLASSES].requires_grad_(True)
+    values, seen = torch.randn(ROWS, CLASSES), []
+
+    def pack(t):
+        return (t, t.dim() == 2)
+
+    def unpack(packed):
+        t, logits = packed
+        if not logits:
+            return t
+        if kind == "dense":
+            out = room[:ROWS * CLASSES].view(ROWS, CLASSES)
+        elif kind == "columns":
+            out = torch.zeros(CLASSES, ROWS).t()
+        else:
+            out = torch.zeros(ROWS, 9)[:, :CLASSES]
+        with torch.no_grad():
+            out.copy_(values)
+        seen.append(out)
+        return out
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        out = functions(z)[name]()
+    forward = next(a[0] for n, a in calls if n in ("rs_token_logprobs", "rs_policy_loss"))
+    assert forward["ld"] == 16 and forward["logits"] == z.data_ptr()
+    torch.autograd.grad(out.sum(), z)
+    desc = next(a[0] for n, a in calls if n.endswith("backward"))
+    assert desc["ld"] == (9 if kind == "pitched" else CLASSES)
+    if kind != "columns":
+        assert desc["logits"] == seen[-1].data_ptr()
+    else:
+        assert desc["logits"] != seen[-1].data_ptr()          # a copy whose rows lie dense
+
+
+def test_saved_logits_that_come_back_as_something_else_are_refused(calls):
+    for other in (torch.zeros(ROWS, CLASSES, dtype=torch.bfloat16), torch.zeros(ROWS - 1, CLASSES), torch.zeros(ROWS, CLASSES + 1), torch.zeros(ROWS)):
+        z = leaf()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other if t.dim() == 2 else t):
+            out = functions(z)["policy"]()
+        with pytest.raises(O._lib.RepSurfHipError, match="saved logits"):
+            torch.autograd.grad(out.sum(), z)

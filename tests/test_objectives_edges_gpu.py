@@ -204,3 +204,33 @@ def test_the_slope_of_pairs_that_are_far_apart(apart, smoothing):
     w, = torch.autograd.grad(ref.logp, ref.z, c)
     ref.check_grad(g, w, torch.float32, c, spread(torch.cat([off, off]) * beta / 2) + 4 * U * c.abs())
     assert (g != 0).any()
+
+
+# ---- saved logits in another layout -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("classes", [13, 5003])
+def test_pitched_logits_that_come_back_dense(classes):
+    """unpacked where they lay, but without their pitch; and by columns"""
+    z, y, off, old, adv, pref = small_case(classes)
+    room = torch.zeros(50 * (classes + 30), device="cuda")
+    pitched = room.view(50, classes + 30)[:, :classes]
+    for name in ("token", "sequence", "preference", "policy"):
+        leaf = z.clone().requires_grad_(True)
+        up = 0.5 * torch.ones_like(losses(leaf, y, off, old, adv, pref)[name]())
+        want, = torch.autograd.grad(losses(leaf, y, off, old, adv, pref)[name](), leaf, up)
+        for dense in (True, False):
+            with torch.no_grad():
+                pitched.copy_(z)
+            leaf = pitched.detach().requires_grad_(True)
+
+            def unpack(t):
+                if t.dim() != 2:
+                    return t
+                out = room[:50 * classes].view(50, classes) if dense else torch.empty(classes, 50, device="cuda").t()
+                with torch.no_grad():
+                    out.copy_(z)
+                return out
+
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                loss = losses(leaf, y, off, old, adv, pref)[name]()
+            got, = torch.autograd.grad(loss, leaf, up)
+            assert torch.equal(got, want), (name, dense)
