@@ -140,7 +140,8 @@ class AdamWArgs(ctypes.Structure):           # rs_adamw_args
                 ("low", P), ("step", P), ("done", P), ("hyper_dev", P), ("hyper", ctypes.c_double * 7), ("clip", P), ("seed", ctypes.c_uint)]
 
 
-_address, _dense, _size = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
+_address, _dense, _size, _type = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.dtype.__get__
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 class _Table:
@@ -356,11 +357,14 @@ class AdamW(Adam):
 
     # ---- the update ---------------------------------------------------------------------------------------------------
     def _tables(self, st, params):
-        """the group's lists (fp32, bf16), rebuilt when an address changed since the last step"""
+        """the group's lists (fp32, bf16), rebuilt when an address, a size or a type changed since the last step"""
         grads = [p.grad for p in params]
-        some = [g for g in grads if g is not None]
-        plan = (list(map(_address, params)), list(map(_address, some)), list(map(_size, params)),          # (a gradient has its parameter's size)
-                len(some) == len(params) or [g is None for g in grads])
+        try:
+            at, some = list(map(_address, grads)), grads
+        except TypeError:          # (None among them)
+            some = [g for g in grads if g is not None]
+            at = list(map(_address, some)) + [g is None for g in grads]
+        plan = (list(map(_address, params)), list(map(_size, params)), list(map(_type, params)), at, list(map(_type, some)))      # (a gradient has its parameter's shape)
         if plan == st["plan"] and all(map(_dense, some)) and all(map(_dense, params)):
             return st["tables"], None
         rows, keep, seen = ([], []), [], set()
@@ -368,6 +372,8 @@ class AdamW(Adam):
             if g is None or p.numel() == 0:
                 continue
             self._check_param(p, st["step"].device)
+            if p.dtype == torch.bfloat16 and "low" not in st["flat"]:
+                raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: a parameter became bf16 after its state was made, without a master's low half")
             if p.numel() != st["sizes"][i] or g.shape != p.shape:
                 raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: a parameter has another size than its state or its gradient")
             if g.layout != torch.strided or g.dtype != p.dtype:
@@ -376,14 +382,13 @@ class AdamW(Adam):
                 raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: two parameters of a group share their memory")
             seen.add(p.data_ptr())
             if not g.is_contiguous():
-                g = g.contiguous()
+                g = g.detach().contiguous()
                 keep.append(g)
             rows[p.dtype == torch.bfloat16].append((p.data_ptr(), g.data_ptr(), p.numel(), st["at"][i], i))
         tables = [(bf16, _Table(r)) for bf16, r in enumerate(rows) if r]
         st["plan"], st["tables"] = (None, None) if keep else (plan, tables)
         return tables, keep
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -402,7 +407,7 @@ class AdamW(Adam):
             work.append((gi, group, st) + self._tables(st, params))
         if not work:
             return loss
-        if dev.index != torch.cuda.current_device():
+        if dev.index != _current_device():
             with torch.cuda.device(dev):
                 self._launch(work, dev)
         else:

@@ -36,3 +36,55 @@ def test_it_takes_its_own_state_back(on_the_cpu, bits, dtype):
         assert s.keys() == got["state"][i].keys()
         for k, v in s.items():
             assert torch.equal(v, got["state"][i][k]), (i, k)
+
+
+def tables_of(opt, st):
+    tables, _ = opt._tables(st, opt.param_groups[0]["params"])
+    return [(bf16, list(t.p), list(t.n)) for bf16, t in tables]
+
+
+def test_lists_follow_the_parameters_types(on_the_cpu):
+    """parameters and gradients whose memory stays where it is while its type changes: another list, or a refusal"""
+    opt, st = made(32, (40,), (30,))
+    a, b = opt.param_groups[0]["params"]
+    words, grads = [p.detach().clone() for p in (a, b)], [torch.zeros(40), torch.zeros(30)]
+
+    def give(kinds):
+        for p, w, g, kind in zip((a, b), words, grads, kinds):
+            p.grad = None
+            p.data = w.view(kind)[:w.numel()]
+            p.grad = g.view(kind)[:w.numel()]
+
+    f, h = torch.float32, torch.bfloat16
+    give((f, f))
+    first = tables_of(opt, st)
+    assert first == [(0, [a.data_ptr(), b.data_ptr()], [40, 30])] and tables_of(opt, st) == first
+    give((f, h))
+    with pytest.raises(optim._lib.RepSurfHipError, match="became bf16"):
+        opt._tables(st, [a, b])
+    give((f, f))
+    assert tables_of(opt, st) == first
+    opt = optim.AdamW([torch.nn.Parameter(torch.zeros(40, dtype=h)), torch.nn.Parameter(torch.zeros(30))])
+    a, b = opt.param_groups[0]["params"]
+    st = opt._group_state(0, opt.param_groups[0], torch.device("cpu"))
+    give((h, f))
+    assert tables_of(opt, st) == [(0, [b.data_ptr()], [30]), (1, [a.data_ptr()], [40])]
+    give((f, f))
+    assert tables_of(opt, st) == [(0, [a.data_ptr(), b.data_ptr()], [40, 30])]
+    give((h, f))
+    assert tables_of(opt, st) == [(0, [b.data_ptr()], [30]), (1, [a.data_ptr()], [40])]
+
+
+def test_a_gradient_of_another_type_is_refused(on_the_cpu):
+    opt, st = made(32, (40,))
+    p, g = opt.param_groups[0]["params"][0], torch.zeros(40)
+    p.grad = g
+    tables_of(opt, st)
+    if not hasattr(p, "grad_dtype"):
+        pytest.skip("gradients have their parameter's type here")
+    p.grad = None
+    p.grad_dtype = torch.bfloat16
+    p.grad = g.view(torch.bfloat16)[:40]
+    assert p.grad.data_ptr() == g.data_ptr()
+    with pytest.raises(optim._lib.RepSurfHipError, match="parameter's type"):
+        opt._tables(st, [p])
