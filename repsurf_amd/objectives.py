@@ -44,15 +44,15 @@ class PolicyDesc(ctypes.Structure):          # rs_policy
                 ("loss", P), ("stats", P), ("logp", P), ("dlogits", P), ("coef", P), ("stat", P), ("scratch", P)]
 
 
-def _no_tangent(t):
+def _no_tangent(*tensors):
     """forward-mode derivatives are refused: nothing here would carry a tangent on"""
-    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:      # (below 0: no level is entered)
-        raise NotImplementedError("objectives: forward-mode derivatives are not offered")
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("objectives: forward-mode derivatives are not offered")          # (a level below 0: none is entered)
 
 
-def _logits(logits, target, offset):
+def _logits(logits, target, offset, *data):
     """checks, and the tensors as the kernels take them"""
-    _no_tangent(logits)
+    _no_tangent(logits, *data)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"objectives: logits must be (rows, classes), got {tuple(logits.shape)}")
     if logits.dtype not in _TYPES:
@@ -86,7 +86,6 @@ def _as(t, dtype):
 
 
 def _values(name, t, shape, logits):
-    _no_tangent(t)
     if t.shape != shape:
         raise ValueError(f"objectives: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != logits.device:
@@ -124,11 +123,12 @@ def _backward(ctx, logits, target, offset, work, coef, gout, flags=0, out=None):
     floats from its start; coef: an address in it, or of a tensor that the caller holds.  (Autograd runs this on a thread of its own, whose every
     line costs twice what it costs elsewhere.)"""
     desc = ctx.desc
-    if (*logits.shape, _TYPES.get(logits.dtype)) != (desc.rows, desc.classes, desc.type):
+    rows, classes = logits.shape if logits.dim() == 2 else (-1, -1)
+    if rows != desc.rows or classes != desc.classes or _TYPES.get(logits.dtype) != desc.type:
         raise _lib.RepSurfHipError("objectives: the saved logits came back with another shape or type")
-    if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)          # (also where the logits have a pitch)
     logits, desc.ld = _pitched(logits)
+    if out is None:
+        out = torch.empty_like(logits)          # (contiguous also where the logits have a pitch)
     desc.logits, desc.target = logits.data_ptr(), target.data_ptr()
     if offset is not None:
         desc.offset = offset.data_ptr()
@@ -270,7 +270,7 @@ def preference_loss(logits, target, offset, ref_logps, beta=0.1, label_smoothing
         loss = mean of -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h).
     ref_logps (2 P,): sequence_logprobs of the reference model's logits (same `average`).
     -> PreferenceLoss(loss, chosen_rewards, rejected_rewards); the rewards (P,) are r, detached."""
-    logits, target, offset = _logits(logits, target, offset)
+    logits, target, offset = _logits(logits, target, offset, ref_logps)
     n = offset.numel()
     if n % 2:
         raise ValueError(f"preference_loss: {n} sequences are no pairs")
@@ -295,7 +295,7 @@ class _Policy(Function):
         count_at = scratch + 4 * room
         stat = count_at + 4 * counts
         coef = stat + 8 * rows
-        d = torch.empty_like(logits, memory_format=torch.contiguous_format) if grad else None
+        d = torch.empty_like(logits) if grad else None
         held = grad and rows > 0
         desc = _desc(logits, target, ignore_index, offset)
         p = PolicyDesc(old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr(), int(adv.dim() == 2), int(token_mean), low, high, kl_coef,
@@ -334,7 +334,7 @@ def policy_loss(logits, target, old_logp, advantages, ref_logp=None, offset=None
     whose ratio was cut off, both weighted like the loss.
     One pass over the logits: the gradient is formed with the loss, and `loss.backward()` hands it out (a pass with another upstream
     gradient than 1 computes it again from the logits, with one rounding)."""
-    logits, target, offset = _logits(logits, target, offset)
+    logits, target, offset = _logits(logits, target, offset, old_logp, advantages, ref_logp)
     rows = logits.shape[0]
     if reduction not in ("token", "sequence"):
         raise ValueError(f"policy_loss: reduction={reduction!r} ('token' or 'sequence')")

@@ -76,9 +76,13 @@ def test_forward_mode_is_refused():
                          lambda: O.policy_loss(dual, y, one, one)):
                 with pytest.raises(NotImplementedError):
                     call()
-        with pytest.raises(NotImplementedError):
-            O._values("data", fw.make_dual(one, one), (ROWS,), leaf())
-        assert O._values("data", one, (ROWS,), leaf()) is one
+        z, dual, two_dual = leaf(), fw.make_dual(one, one), fw.make_dual(two, two)
+        for call in (lambda: O.policy_loss(z, y, dual, one), lambda: O.policy_loss(z, y, one, dual), lambda: O.policy_loss(z, y, one, one, ref_logp=dual),
+                     lambda: O.preference_loss(z, y, off, two_dual)):
+            with pytest.raises(NotImplementedError):
+                call()
+        with pytest.raises(O._lib.RepSurfHipError, match="HIP device"):          # no tangent: it goes on as far as it can on the CPU
+            O.policy_loss(z, y, one, one)
 
 
 @pytest.mark.parametrize("name", NAMES)
