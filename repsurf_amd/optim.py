@@ -318,6 +318,10 @@ class AdamW(Adam):
                 for name, v in saved.items():
                     if name in ("exp_avg", "exp_avg_sq", "low") and tuple(v.shape) != tuple(p.shape):
                         raise ValueError(f"AdamW.load_state_dict: {name} of parameter {k} has shape {tuple(v.shape)}, the parameter {tuple(p.shape)}")
+                    if name.endswith("_exponent") and tuple(v.shape) != ((p.numel() + BLOCK - 1) // BLOCK,):
+                        raise ValueError(f"AdamW.load_state_dict: {name} of parameter {k} has shape {tuple(v.shape)}, one per {BLOCK} elements are needed")
+                if ("exp_avg" in saved) != ("exp_avg_sq" in saved):
+                    raise ValueError(f"AdamW.load_state_dict: parameter {k} has one moment without the other")
         # state_dict() hands out views of the buffers that are written below: such values are read whole before anything is
         own = {buf.untyped_storage().data_ptr() for st in self._dev.values() for buf in st["flat"].values()}
         kept = lambda v: v.clone() if torch.is_tensor(v) and v.untyped_storage().data_ptr() in own else v      # noqa: E731

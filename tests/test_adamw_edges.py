@@ -88,3 +88,27 @@ def test_a_gradient_of_another_type_is_refused(on_the_cpu):
     assert p.grad.data_ptr() == g.data_ptr()
     with pytest.raises(optim._lib.RepSurfHipError, match="parameter's type"):
         opt._tables(st, [p])
+
+
+def test_state_that_does_not_fit_is_refused_before_anything_is_written(on_the_cpu):
+    opt, st = made(8, (300, 5), (256,))
+    good = opt.state_dict()
+    before = {k: v.clone() for k, v in st["flat"].items()}
+
+    def spoiled(i, **kw):
+        state = {k: dict(v) for k, v in good["state"].items()}
+        for k, v in kw.items():
+            if v is None:
+                del state[i][k]
+            else:
+                state[i][k] = v
+        return {"state": state, "param_groups": [dict(good["param_groups"][0], lr=0.5)]}
+
+    byte = lambda *n: torch.zeros(n, dtype=torch.uint8)      # noqa: E731
+    for bad, text in ((spoiled(0, exp_avg_exponent=byte(1)), "exponent"), (spoiled(0, exp_avg_sq_exponent=byte(7)), "exponent"),
+                      (spoiled(1, exp_avg_exponent=byte(2)), "exponent"), (spoiled(1, exp_avg_exponent=torch.tensor(3, dtype=torch.uint8)), "exponent"),
+                      (spoiled(1, exp_avg_sq=None, exp_avg_sq_exponent=None), "without the other"), (spoiled(0, exp_avg=None), "without the other")):
+        with pytest.raises(ValueError, match=text):
+            opt.load_state_dict(bad)
+        assert opt.param_groups[0]["lr"] == good["param_groups"][0]["lr"] and st["step"].tolist() == [100, 101]
+        assert all(torch.equal(v, before[k]) for k, v in st["flat"].items())
