@@ -239,6 +239,8 @@ class _SequenceLogprobs(Function):
 def sequence_logprobs(logits, target, offset, ignore_index=-100, average=False):
     """(B,) fp32: the sum of token_logprobs over every sequence of a packed batch, or (average) their mean over the rows that count; 0 for
     a sequence without any.  Differentiable in the logits."""
+    if offset is None:
+        raise ValueError("sequence_logprobs: needs offset, the (B,) running row ends")
     logits, target, offset = _logits(logits, target, offset)
     return _run(_SequenceLogprobs, logits, target, offset, ignore_index, average)
 
@@ -270,6 +272,8 @@ def preference_loss(logits, target, offset, ref_logps, beta=0.1, label_smoothing
         loss = mean of -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h).
     ref_logps (2 P,): sequence_logprobs of the reference model's logits (same `average`).
     -> PreferenceLoss(loss, chosen_rewards, rejected_rewards); the rewards (P,) are r, detached."""
+    if offset is None:
+        raise ValueError("preference_loss: needs offset, the (B,) running row ends")
     logits, target, offset = _logits(logits, target, offset, ref_logps)
     n = offset.numel()
     if n % 2:

@@ -132,3 +132,10 @@ def test_saved_logits_that_come_back_as_something_else_are_refused(calls):
             out = functions(z)["policy"]()
         with pytest.raises(O._lib.RepSurfHipError, match="saved logits"):
             torch.autograd.grad(out.sum(), z)
+
+
+def test_sequences_need_their_offset():
+    y = torch.zeros(ROWS, dtype=torch.long)
+    for call in (lambda: O.sequence_logprobs(leaf(), y, None), lambda: O.preference_loss(leaf(), y, None, torch.zeros(2))):
+        with pytest.raises(ValueError, match="offset"):
+            call()
