@@ -697,6 +697,9 @@ typedef struct rs_policy {
 #define RS_POLICY_GROUPS 8192
 int rs_policy_loss(const rs_logits *l, const rs_policy *p, void *stream);
 
+/* *id (HOST) = the number of the capture that the stream is part of, 0 outside of captures */
+int rs_capture_id(unsigned long long *id, void *stream);
+
 /* Measurement aid (round 6): one-thread launch that stores the device's constant-rate wall clock (s_memrealtime) in *dst when it runs;
  * rs_timestamp_khz() = ticks per millisecond.  bench.py brackets a launch inside the step's replayed hipGraph with two of them (HIP
  * events cannot be recorded inside a replayed graph on this runtime).  Not used by the product path. */

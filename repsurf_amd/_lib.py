@@ -101,6 +101,7 @@ SIGNATURES = {
     "rs_sequence_sums": [P, P, c_int, P, P, P, P],
     "rs_preference_pairs": [c_int, P, P, P, ctypes.c_double, ctypes.c_double, P, P, P, P],
     "rs_policy_loss": [P, P, P],
+    "rs_capture_id": [P, P],
     "rs_ballquery_grid_build": [c_int, c_int, c_float, P, P, P],
     "rs_ballquery_grid_query": [c_int, c_int, c_int, c_float, c_int, P, P, P, P, P],
 }

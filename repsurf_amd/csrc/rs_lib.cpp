@@ -39,3 +39,13 @@ extern "C" int rs_device_info(int *cu_count, int *wave_size, int *lds_bytes, cha
   if (arch && arch_len > 0) { strncpy(arch, p.gcnArchName, arch_len - 1); arch[arch_len - 1] = 0; }
   return RS_OK;
 }
+
+extern "C" int rs_capture_id(unsigned long long *id, void *stream) {
+  RS_REQUIRE(id, "rs_capture_id: null pointer");
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  *id = 0;
+  const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &status, id);
+  if (e != hipSuccess) { rs_set_error("rs_capture_id: %s", hipGetErrorString(e)); return RS_ERR_HIP_BASE + (int)e; }
+  if (status == hipStreamCaptureStatusNone) *id = 0;
+  return RS_OK;
+}

@@ -118,6 +118,18 @@ def _call(device, name, *args):
             _lib.call(name, *args, _lib.current_stream())
 
 
+def _capture(device):
+    """the number of the capture that the current stream of a device is part of; 0: of none"""
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return _capture(device)
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    number = ctypes.c_ulonglong()
+    _lib.call("rs_capture_id", ctypes.byref(number), _lib.current_stream())
+    return number.value
+
+
 def _backward(ctx, logits, target, offset, work, coef, gout, flags=0, out=None):
     """from the tensors as autograd hands them back (a hook may have moved them, to another pitch too); the rows' stat lies in `work`, ctx.stat
     floats from its start; coef: an address in it, or of a tensor that the caller holds.  (Autograd runs this on a thread of its own, whose every
@@ -308,7 +320,7 @@ class _Policy(Function):
         _call(logits.device, "rs_policy_loss", ctypes.byref(desc), ctypes.byref(p))
         if grad:
             _keep(ctx, desc, (stat - at) // 4, logits, target, work, offset)
-            ctx.d = d
+            ctx.d, ctx.capture = d, _capture(logits.device)
         ctx.mark_non_differentiable(logp, stats)
         return loss, logp, stats
 
@@ -317,8 +329,10 @@ class _Policy(Function):
     def backward(ctx, g, *_):
         logits, target, work, offset = ctx.saved_tensors
         d = ctx.d
-        first = d is not None
         ctx.d = None                       # handed out once: a second pass over a retained graph computes it again
+        if d is not None and ctx.capture != _capture(logits.device):
+            d = None                       # so does one that is replayed apart from the forward pass, which is each time a pass of its own
+        first = d is not None
         if first and head._unit:
             one = head._unit.get(str(logits.device))
             if one is not None and g.data_ptr() == one.data_ptr():          # loss.backward(unit_gradient(device))

@@ -17,6 +17,7 @@ def calls(monkeypatch):
 
     monkeypatch.setattr(O, "_call", record)
     monkeypatch.setitem(O._bad, None, 0)
+    monkeypatch.setattr(O, "_capture", lambda device: 0)
     return made
 
 

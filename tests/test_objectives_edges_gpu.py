@@ -234,3 +234,69 @@ def test_pitched_logits_that_come_back_dense(classes):
                 loss = losses(leaf, y, off, old, adv, pref)[name]()
             got, = torch.autograd.grad(loss, leaf, up)
             assert torch.equal(got, want), (name, dense)
+
+
+# ---- a backward pass captured without its forward pass --------------------------------------------------------------------
+@pytest.mark.parametrize("name", ["token", "sequence", "preference", "policy"])
+@pytest.mark.parametrize("classes", [13, 5003])
+def test_a_captured_backward_pass_of_an_eager_forward_pass(name, classes):
+    """Replays with upstream gradients of 0.5, 1, 2 and 1 again, each against an eager pass; what a replay returned may be overwritten in
+    between.  The logits are no leaf: nothing is accumulated in the graph."""
+    z, y, off, old, adv, pref = small_case(classes)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = z.clone().requires_grad_(True) * 1.0
+        f = losses(x, y, off, old, adv, pref)[name]
+        warm = f()
+        up = torch.ones_like(warm)
+        torch.autograd.grad(warm, x, up, retain_graph=True)
+        out = f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        g, = torch.autograd.grad(out, x, up, retain_graph=True)
+    for k in (0.5, 1.0, 2.0, 1.0):
+        with torch.cuda.stream(side):
+            up.fill_(k)
+            graph.replay()
+            got = g.clone()
+            g.zero_()
+            want, = torch.autograd.grad(warm, x, up, retain_graph=True)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), k
+
+
+@pytest.mark.parametrize("classes", [13, 5003])
+def test_forward_and_backward_passes_in_graphs_of_their_own(classes):
+    """the second graph twice for each replay of the first, on new logits"""
+    z, y, off, old, adv, pref = small_case(classes)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = z.clone().requires_grad_(True)
+        w = x * 1.0
+        f = losses(w, y, off, old, adv, pref)["policy"]
+        up = torch.ones_like(f())
+        torch.autograd.grad(f(), w, up)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=side):
+        out = f()
+    with torch.cuda.graph(second, stream=side, pool=first.pool()):
+        g, = torch.autograd.grad(out, w, up, retain_graph=True)
+    for k in range(3):
+        with torch.cuda.stream(side):
+            with torch.no_grad():
+                w.copy_(logits_of(50, classes, torch.float32, seed=20 + k))
+            first.replay()
+            again = w.detach().clone().requires_grad_(True)
+            for factor in (0.5, 1.0, 2.0):
+                up.fill_(factor)
+                second.replay()
+                got = g.clone()
+                g.zero_()
+                loss = losses(again, y, off, old, adv, pref)["policy"]()
+                want, = torch.autograd.grad(loss, again, up)
+                assert torch.equal(out, loss) and torch.equal(got, want), (k, factor)
+        torch.cuda.synchronize()
