@@ -7,8 +7,11 @@ LIBDIR := repsurf_amd/lib
 # operation by operation; fused multiply-adds appear only where written (rs_fma).
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off \
             -fhip-fp32-correctly-rounded-divide-sqrt -munsafe-fp-atomics -Wall -Wno-unused-function
-# No packed-fp32 instructions anywhere: some of their forms give other results beside another kernel's MFMAs (see below).  At no cost: the
-# classification step 1.218 ms with and 1.217 ms without them, the segmentation step 3.314 and 3.319 ms (runs of each in turn, one GPU).
+# No packed-fp32 instructions anywhere: some of their forms give other results beside another kernel's MFMAs (see below).  What it costs: the
+# graphed steps nothing (classification 1.218 ms with and 1.217 ms without them, segmentation 3.314 and 3.319 ms, runs of each in turn, one GPU)
+# -- farthest-point sampling, whose distance update they halved, runs hidden there; by itself it is 8 to 11 % slower up to 1 024 points a cloud
+# (32 x 1024 -> 512: 252 and 279 us) and 6 to 8 % in packed batches; ball query, kNN and the constructor's kernels are as they were
+# (profiles/objectives_adamw/without_packed_fp32.csv).
 HIPFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 SRCS := $(CSRC)/rs_lib.cpp $(CSRC)/fps.hip $(CSRC)/ballquery.hip $(CSRC)/knn_umbrella.hip $(CSRC)/knn_wide.hip \
         $(CSRC)/group.hip $(CSRC)/interp.hip $(CSRC)/seg_geom.hip $(CSRC)/scene_knn.hip $(CSRC)/grid_knn.hip $(CSRC)/mlp.hip $(CSRC)/umbrella_mlp.hip $(CSRC)/umbrella_mfma.hip $(CSRC)/head.hip $(CSRC)/adam.hip $(CSRC)/adamw.hip $(CSRC)/logits.hip

@@ -602,7 +602,7 @@ int rs_adam_step(const rs_adam_table *t, double *hyper, int *step, int *done, in
  * An element is rounded up with the probability of the part that is cut off, by 16 bits of a hash of (seed, t, its block, its place in
  * the block); a positive second moment keeps at least c = 1.  Zeroed buffers are the initial state.
  * bf16 parameters: `low` (flat, like the moments) holds what the fp32 master has below the parameter: master bits =
- * (parameter bits << 16) + low. */
+ * (parameter bits << 16) + low, a signed number of 16 bits.  So the parameter is its master rounded to nearest, halves away from zero. */
 typedef struct rs_adamw_list {   /* HOST arrays of `count` entries; nothing is kept after the call */
   int count;
   void *const *p;                /* parameters, updated in place (contiguous, aligned to an element) */

@@ -284,10 +284,14 @@ __device__ __forceinline__ void lg_partial(const Policy &P, const double *add, i
 // Rows of up to 4096 classes: LANES neighbouring lanes hold a row in NV vectors of 8 per lane; one read, one write.  A team takes SUB rows
 // before the fp64 steps, which its first SUB lanes then do for a row each: with 13 classes (2 lanes, 2 rows) every lane of a wave works
 // on a row of its own.  The policy loss is bound by those steps (some 300 instructions in fp64) and by the registers that its rows stay
-// in; four waves per SIMD and SUB * NV = 4 measured best (SUB * NV = 8 with two waves: 13..18 % slower).  Against a workgroup per row
-// (long_kernel): 2048 classes 192 against 404 us, 4096 191 against 239 (65536 and 32768 rows in bf16), so the border is the 8 vectors
-// that a lane can hold.  Measured: policy loss, fp32, 65536 x 2048 247 us = 4.3 TB/s, 1048576 x 40 173 us; backward 2097152 x 13 96 us =
-// 2.3 TB/s (rows of 52 bytes, two lanes each); log-probabilities 32768 x 4096 in bf16 46 us = 5.8 TB/s.
+// in; four waves per SIMD and SUB * NV = 4 measured best over all lengths (SUB * NV = 8 with two waves: 13..18 % slower).  Against a workgroup
+// per row (long_kernel): 2048 classes 171 against 294 us, 4096 152 against 167 (65536 and 32768 rows in bf16), so the border is the 8
+// vectors that a lane can hold (in fp32 4096 classes are the other way round, 273 against 255).  Measured: policy loss, fp32, 65536 x 2048
+// 246 us = 4.4 TB/s, 1048576 x 40 169 us; backward 2097152 x 13 81 us = 2.7 TB/s (rows of 52 bytes, two lanes each); log-probabilities
+// 32768 x 4096 in bf16 46 us = 5.9 TB/s.
+// What four waves cost: in fp32 the policy loss spills 40 registers at <64, 8>, 17 at <64, 1>, 4 to 8 at <4..32, 1> (in 16 bits 2
+// at <64, 8>); with three waves none does.  Three against four: 32768 x 4096 239 and 273 us, 262144 x 500 443 and 483 -- but 262144 x 250 229 and 196, 524288 x 100 221 and
+// 188, 524288 x 64 120 and 108, 131072 x 1000 330 and 287.
 template <typename T, int MODE, int LANES, int NV>
 __global__ void __launch_bounds__(256, MODE == LG_POLICY ? 4 : 1)
 short_kernel(Rows R, Policy P, Outs O) {
@@ -384,7 +388,7 @@ __device__ __forceinline__ void lg_step_out(T *__restrict__ dz, int k, unsigned 
 }
 
 // The logits in front of a row's first 16-byte border, one for each of the first threads: the vectors of rows of an odd number of classes
-// would straddle cache lines otherwise (bf16, 8192 x 50001: log-probabilities 179 us without, 157 us with heads, policy loss 403 and 363).
+// would straddle cache lines otherwise (bf16, 8192 x 50001: log-probabilities 172 us without, 139 us with heads, policy loss 363 and 333).
 template <typename T>
 __device__ __forceinline__ int lg_head(const T *z, int V) {
   const int n = (int)((16 - ((size_t)z & 15)) & 15) / (int)sizeof(T);
@@ -394,10 +398,11 @@ __device__ __forceinline__ int lg_head(const T *z, int V) {
 // Long rows, one workgroup each, LDS for what its waves tell each other.  HELD (the policy loss): the row stays in registers between its
 // sum and its gradient, at most NV steps of 8 logits per thread and a tail.  Otherwise chunks of NV steps are taken in turn: their loads
 // are all in flight before the first is used, and the running maximum is corrected once per chunk.
-// Bound by memory: policy loss in bf16 8192 x 32768 240 us, 8192 x 65536 444 us, 8192 x 50001 360 us (4.5..4.8 TB/s), fp32 8192 x 32768 429 us
-// (5.0); log-probabilities 8192 x 65536 in bf16 180 us = 5.9 TB/s.  256 threads leave room for two or three rows on a CU, whose loads, sums
-// and stores overlap (1024 threads, one row: 2.0..2.8 TB/s); at 131072 classes one row is all that fits (3.9 TB/s).  Held against read twice
-// (HELD false, 262144 classes: 3.4 TB/s), a row costs a third less traffic.
+// Bound by memory: policy loss in bf16 8192 x 32768 219 us, 8192 x 65536 433 us, 8192 x 50001 333 us (4.9..5.0 TB/s), fp32 8192 x 32768 425 us
+// (5.1); log-probabilities 8192 x 65536 in bf16 183 us = 5.9 TB/s.  256 threads leave room for two or three rows on a CU, whose loads, sums
+// and stores overlap (1024 threads, one row: 395, 574 and 519 us, 529 in fp32); at 131072 classes one row is all that fits (4096 rows 557 us,
+// 3.9 TB/s).  Held against read twice (HELD false: 263, 500 and 396 us, 494 in fp32, 604 at 131072; 262144 classes, which are always read
+// twice, 3.4 TB/s), a row costs a third less traffic.
 // (WAVES per SIMD bound the registers: left alone, the compiler interleaves the steps until two waves are all that fits)
 template <typename T, int MODE, int THREADS, int NV, bool HELD, int WAVES>
 __global__ void __launch_bounds__(THREADS, WAVES)
@@ -522,7 +527,7 @@ long_kernel(Rows R, Policy P, Outs O) {
 }
 
 // backward pass of long rows: a workgroup takes 256 * 8 * NV logits of a row at a time, whatever row they are of.  Bound by memory: 8192 x
-// 65536 in bf16 379 us = 5.7 TB/s, fp32 8192 x 32768 389 us = 5.5 TB/s
+// 65536 in bf16 373 us = 5.8 TB/s, fp32 8192 x 32768 382 us = 5.6 TB/s
 template <typename T, int NV>
 __global__ void __launch_bounds__(256, 7)
 long_back_kernel(Rows R, Outs O, int parts) {
@@ -559,7 +564,7 @@ long_back_kernel(Rows R, Outs O, int parts) {
   }
 }
 
-// Few long rows: a row in `parts` pieces, (M, s) of each ...  (one row of 100001 classes in bf16: 3.5 + 2.1 us, against 13.7 us by one
+// Few long rows: a row in `parts` pieces, (M, s) of each ...  (one row of 100001 classes in bf16: 3.3 + 2.0 us, against 9.5 us by one
 // workgroup; the launches' own time bounds both)
 template <typename T, int NV>
 __global__ void __launch_bounds__(256)
@@ -759,19 +764,20 @@ int launch_rows(const rs_logits *l, const Rows &R, const Policy &P, const Outs &
 #define LG_RUN_LONG(TH, N, H, WV) { const int g = lesser(R.rows, MODE == LG_POLICY ? RS_POLICY_GROUPS : LG_LONG_GRID); hipLaunchKernelGGL((long_kernel<T, MODE, TH, N, H, WV>), dim3(g), dim3(TH), 0, st, R, P, O); return g; }
     if constexpr (MODE == LG_POLICY) {       // (without a gradient too: the loss has the same bits either way)
       constexpr int K = sizeof(T) / 2;       // 8 logits: 4 or 8 registers of a thread
-      // (in 16 bits 128 threads to a row while 16 steps hold it: two waves share its fp64 steps and barriers, not four.  32768 x 5000 210 us
-      // against 272, 16384 x 8192 137 against 155, 16384 x 16000 234 against 248; 8192 x 32768 223 against 217)
+      // (in 16 bits 128 threads to a row while 16 steps hold it: two waves share its fp64 steps and barriers, not four.  Against 256 threads:
+      // 32768 x 5000 198 and 264 us, 16384 x 8192 128 and 141, 16384 x 16000 229 and 242; with 32 steps 8192 x 32768 255 and 219.
+      // They spill 7 to 9 registers for it.)
       if constexpr (K == 1) {
         if (V < 9216) LG_RUN_LONG(128, 8, true, 5)
         if (V < 17408) LG_RUN_LONG(128, 16, true, 4)
       } else {
-        if (V < 5120) LG_RUN_LONG(128, 4, true, 5)        // 16384 x 5000 158 us against 169; with 8 steps 16384 x 8192 229 against 222
+        if (V < 5120) LG_RUN_LONG(128, 4, true, 5)        // 16384 x 5000 156 us against 168; with 8 steps 16384 x 8192 229 against 218
         if (V < 10240) LG_RUN_LONG(256, 4, true, 4)
         if (V < 18432) LG_RUN_LONG(256, 8, true, 3)
       }
       if (V < 34816) LG_RUN_LONG(256, 16, true, K == 1 ? 3 : 2)
       if constexpr (K == 1) {
-        if (V < 51200) LG_RUN_LONG(256, 24, true, 3)
+        if (V < 51200) LG_RUN_LONG(256, 24, true, 3)      // three rows on a CU, with 32 steps two: 8192 x 40001 267 us against 304, x 50001 333 against 355
         if (V < 67584) LG_RUN_LONG(256, 32, true, 2)
         if (V < 135168) LG_RUN_LONG(512, 32, true, 2)
       } else {

@@ -62,7 +62,8 @@ __device__ __forceinline__ float pack_bf16(float lo, float hi) {
 // so h + m + l differs from x by at most the last rounding: 2^-8 of 2^-16 |x|.
 constexpr bool RS_SPLIT = RS_MLP_TU == 4;
 __device__ __forceinline__ void split_bf16(float x0, float x1, float (&d)[3]) {
-  // (the two residual subtractions of a pair as ONE v_pk_add_f32 each -- exact either way: 9 instead of 11 VALU per pair)
+  // (the two residual subtractions of a pair as two scalar ones each, 11 VALU per pair: the library is built without packed-fp32 instructions,
+  // with which they would be 9; exact either way)
   d[0] = pack_bf16(x0, x1);
   unsigned u = __float_as_uint(d[0]);
   const f32x2 x = {x0, x1};

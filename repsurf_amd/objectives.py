@@ -351,7 +351,7 @@ def policy_loss(logits, target, old_logp, advantages, ref_logp=None, offset=None
     -> PolicyLoss(loss, logp (rows,), kl, clip_fraction); the last three are detached: x, the mean of exp(d) - 1 - d and the share of rows
     whose ratio was cut off, both weighted like the loss.
     One pass over the logits: the gradient is formed with the loss, and `loss.backward()` hands it out (a pass with another upstream
-    gradient than 1 computes it again from the logits, with one rounding)."""
+    gradient than 1, a second one, and one captured without its forward pass compute it again from the logits, with one rounding)."""
     logits, target, offset = _logits(logits, target, offset, old_logp, advantages, ref_logp)
     rows = logits.shape[0]
     if reduction not in ("token", "sequence"):

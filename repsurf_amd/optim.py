@@ -163,7 +163,8 @@ class AdamW(Adam):
     csrc/adamw.hip: the optimizer that the reference's segmentation loop builds (segmentation/tool/train.py).
 
     Parameters are contiguous tensors in fp32, or in bf16 -- these keep, beside the moments, the 16 bits that their fp32 master has below
-    them (`low`), so a step smaller than bf16's spacing is not lost; a parameter that is written from outside moves its master with it.
+    them (`low`), so a step smaller than bf16's spacing is not lost; a parameter that is written from outside moves its master with it.  Such a
+    parameter is its master rounded to nearest, halves away from zero (torch: to even): 16 signed bits hold what is below it.
     state_bits=8 holds both moments in one byte per element and one exponent per 256 (include/repsurf_hip.h has the format): 4 bytes
     of state traffic per parameter instead of 16.  Values are rounded stochastically by a fixed function of (seed, step, element): the
     same run gives the same bits.  max_grad_norm=x multiplies every gradient by min(1, x / (norm + 1e-6)), norm being that of all
@@ -172,7 +173,8 @@ class AdamW(Adam):
 
     Every parameter counts its own steps, on the device: one without a gradient is left out and its bias correction waits, and a
     captured step (graph.GraphedStep, graph.TrainLoopStep) counts its replays.  Hyper-parameters ride in an eager step's launch; a
-    captured one reads them from device memory -- `sync_hyper()` before a replay, as the graphed steps do.
+    captured one reads them from device memory -- `sync_hyper()` before a replay, as the graphed steps do (max_grad_norm, the seed and
+    whether gradients are clipped at all stay what they were at the capture).
 
     The moments of a group are slices of flat buffers (`flat_state`), every tensor at a multiple of 256 elements."""
 
