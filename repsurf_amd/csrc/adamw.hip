@@ -35,6 +35,7 @@ constexpr int AW_SQ_CHUNK = 8192;         // gradients a workgroup squares at a 
 constexpr int AW_MAX = 80;                // tensors per launch: the table rides in the kernel arguments
 constexpr int AW_COUNTS = RS_ADAMW_DONE / 16 - 1;      // counters of finished workgroups, below the one of all
 constexpr int AW_FIELD_M = 14, AW_FIELD_V = 30;
+constexpr float AW_EPS = 1e-9f;           // (1e-19 over sqrt(1 - b2^t), 3e-18 at b2 = 0.999, is below half a unit of what is larger)
 
 struct AwTable {
   void *p[AW_MAX];
@@ -210,8 +211,13 @@ struct AwBlocks {
         mi[i] = mi[i] + (gi - mi[i]) * S.omb1;
         vi[i] = vi[i] * S.b2 + (S.omb2 * gi) * gi;
         // The device's own root and reciprocal, each off by one unit: the correctly rounded ones are 25 instructions for an error that lr
-        // scales away.  The root takes denormals as zero, so v is raised to the smallest normal number (1e-19 beside eps).
-        const float root = __builtin_amdgcn_sqrtf(fmaxf(vi[i], 1.17549435e-38f));
+        // scales away.  The root takes denormals as zero, so v is raised to the smallest normal number (1e-19 beside eps); beside an eps that
+        // does not cover that, denormals are taken 2^64 higher (a vanished v is the smallest of them: no gradient and no eps is no step).
+        float root;
+        if (S.eps < AW_EPS) {
+          const bool small = vi[i] < 1.17549435e-38f;
+          root = __builtin_amdgcn_sqrtf(small ? fmaxf(vi[i], 1.40129846e-45f) * 0x1p64f : vi[i]) * (small ? 0x1p-32f : 1.f);
+        } else root = __builtin_amdgcn_sqrtf(fmaxf(vi[i], 1.17549435e-38f));
         x = rs_fma(-S.step_size, mi[i] * __builtin_amdgcn_rcpf(rs_fma(root, S.inv_bc2, S.eps)), x * S.decay);
         if (!WHOLE && i >= left) mi[i] = vi[i] = x = 0.f;
         if constexpr (BF16) word[i] = aw_word(x); else p[u].w[i] = __float_as_uint(x);

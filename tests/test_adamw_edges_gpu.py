@@ -67,3 +67,32 @@ def test_its_own_state_in_another_order(bits, groups):
         assert torch.equal(opt.state[ps[0]][k], want[1][k]) and torch.equal(opt.state[ps[1]][k], want[0][k])
         assert (opt.state[ps[2]][k] == 0).all()
     assert [float(opt.state_dict()["state"][i]["step"]) for i in range(3)] == [2.0, 2.0, 0.0]
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-20, 1e-12])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_small_eps_beside_small_gradients(eps, dtype):
+    """Second moments down to fp32's smallest numbers, each rounded by at most 2^-150 there (half its spacing), three times a step: the ratio is
+    off by dv / 2 v relatively, beside the bound of the other tests.  A gradient of 0 moves nothing but the decay."""
+    import numpy as np
+    from repsurf_amd.optim import AdamW
+    from tests.test_adamw_gpu import U, Twin, np64
+    hyper = dict(HYPER, eps=eps)
+    n, k = 2100, 3
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device="cuda"))
+    size = torch.logspace(-20.5, -3, n, dtype=torch.float64) * torch.where(torch.arange(n) % 2 == 0, 1.0, -1.0)
+    size[7], size[n - 1] = 0.0, 0.0
+    p.grad = size.to(dtype).cuda()
+    opt, twin = AdamW([p], **hyper), Twin([p], hyper)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        for _ in range(k):
+            opt.step()
+            twin.step([np64(p.grad)])
+    got = opt.unpack_state()["master"][:n].double().cpu().numpy() if dtype == torch.bfloat16 else np64(p)
+    v = twin.v[0]
+    live = np64(p.grad) != 0
+    want = twin.p[0]
+    dv = 3 * k * 2.0 ** -150
+    tol = k * (3 * U * np.abs(want) + hyper["lr"] * (16 * k * U + dv / np.where(live, v, 1.0)))
+    assert (got[~live] == 0).all() and np.isfinite(got).all()
+    assert (v[live].min() < 1e-43) and (np.abs(got - want) <= tol)[live].all()
