@@ -20,7 +20,7 @@
 // Bound by memory: every value is read and written once.  A workgroup takes one chunk of 2048 elements of one tensor, all of its loads in
 // flight at once; workgroups that loop over chunks (2048 of them) were 8..16 % slower, 4096 elements a chunk no faster.  Measured: 100.7 M fp32
 // parameters with fp32 moments 498 us (28 bytes each, 5.7 TB/s), 59.6 M bf16 parameters 272 us (26 bytes, 5.7 TB/s), 268 M fp32 parameters
-// with 8-bit moments 776 us (16 bytes, 5.5 TB/s), 100.7 M bf16 parameters with 8-bit moments 248 us (14 bytes, 5.7 TB/s); 1.48 M in 67
+// with 8-bit moments 763 us (16 bytes, 5.6 TB/s), 100.7 M bf16 parameters with 8-bit moments 239 us (14 bytes, 5.9 TB/s); 1.48 M in 67
 // tensors 9.3 us, most of it the launch, two dependent reads and the counting of finished workgroups (1.2 us).
 #include "rs_common.h"
 #include <math.h>

@@ -176,7 +176,8 @@ class AdamW(Adam):
     captured one reads them from device memory -- `sync_hyper()` before a replay, as the graphed steps do (max_grad_norm, the seed and
     whether gradients are clipped at all stay what they were at the capture).
 
-    The moments of a group are slices of flat buffers (`flat_state`), every tensor at a multiple of 256 elements."""
+    The moments of a group are slices of flat buffers (`flat_state`), every tensor at a multiple of 256 elements; `state_dict()` brings
+    `state[p]["step"]` up to date from the device's counters."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_grad_norm=None, seed=0):
         if state_bits not in (8, 32):
