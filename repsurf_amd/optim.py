@@ -368,8 +368,10 @@ class AdamW(Adam):
         grads = [p.grad for p in params]
         try:
             at, some = list(map(_address, grads)), grads
-        except TypeError:          # (None among them)
+        except (TypeError, RuntimeError):          # (None among them, or one without an address)
             some = [g for g in grads if g is not None]
+            if any(g.layout is not torch.strided for g in some):
+                raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: gradients must be dense and of their parameter's type")
             at = list(map(_address, some)) + [g is None for g in grads]
         plan = (list(map(_address, params)), list(map(_size, params)), list(map(_type, params)), at, list(map(_type, some)))      # (a gradient has its parameter's shape)
         if plan == st["plan"] and all(map(_dense, some)) and all(map(_dense, params)):

@@ -112,3 +112,13 @@ def test_state_that_does_not_fit_is_refused_before_anything_is_written(on_the_cp
             opt.load_state_dict(bad)
         assert opt.param_groups[0]["lr"] == good["param_groups"][0]["lr"] and st["step"].tolist() == [100, 101]
         assert all(torch.equal(v, before[k]) for k, v in st["flat"].items())
+
+
+def test_a_sparse_gradient_is_refused(on_the_cpu):
+    opt, st = made(32, (4, 3), (5,))
+    a, b = opt.param_groups[0]["params"]
+    a.grad, b.grad = torch.sparse_coo_tensor([[0], [1]], [1.0], (4, 3)), torch.zeros(5)
+    for other in (b.grad, None):
+        b.grad = other
+        with pytest.raises(optim._lib.RepSurfHipError, match="dense"):
+            opt._tables(st, [a, b])
