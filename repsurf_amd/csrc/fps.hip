@@ -457,7 +457,9 @@ int fps_dispatch(int blocks, int n_max, int n, int m, const float *xyz, const in
     if (n_dev) positions = n_max >= 1024 ? ((n_max + 1023) / 1024 + 1) * 1024 : 2 * n_max;
   }
   // Waves per workgroup: the loop is a latency chain, so fewer waves (no cross-wave hop, or a short one)
-  // win as long as the per-lane point count stays small (profiles/: RS_FPS_WAVES sweeps).
+  // win as long as the per-lane point count stays small (profiles/: RS_FPS_WAVES sweeps).  Two for 513 .. 1 024 positions: alone, four are
+  // faster since the update's packed-fp32 instructions went (32 x 1024 -> 512: 262 against 279 us), but the classification step, which hides
+  // this launch beside the network, is slower with them (1.224 against 1.217 ms, three runs of each in turn).
   int waves = env_int("RS_FPS_WAVES", 0);
   if (waves <= 0) waves = positions <= 512 ? 1 : (positions <= 1024 ? 2 : (positions <= 4096 ? 4 : (positions <= 8192 ? 8 : 16)));
   int w = 1;
