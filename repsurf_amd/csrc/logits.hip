@@ -289,9 +289,9 @@ __device__ __forceinline__ void lg_partial(const Policy &P, const double *add, i
 // vectors that a lane can hold (in fp32 4096 classes are the other way round, 273 against 255).  Measured: policy loss, fp32, 65536 x 2048
 // 246 us = 4.4 TB/s, 1048576 x 40 169 us; backward 2097152 x 13 81 us = 2.7 TB/s (rows of 52 bytes, two lanes each); log-probabilities
 // 32768 x 4096 in bf16 46 us = 5.9 TB/s.
-// What four waves cost: in fp32 the policy loss spills 40 registers at <64, 8>, 17 at <64, 1>, 4 to 8 at <4..32, 1> (in 16 bits 2
-// at <64, 8>); with three waves none does.  Three against four: 32768 x 4096 239 and 273 us, 262144 x 500 443 and 483 -- but 262144 x 250 229 and 196, 524288 x 100 221 and
-// 188, 524288 x 64 120 and 108, 131072 x 1000 330 and 287.
+// What four waves cost: in fp32 the policy loss spills 40 registers at <64, 8>, 17 at <64, 1>, 4 to 8 at <4..32, 1> (in 16 bits 2 at
+// <64, 8>); with three waves none does.  Three against four: 32768 x 4096 239 and 273 us, 262144 x 500 443 and 483 -- but 262144 x 250
+// 229 and 196, 524288 x 100 221 and 188, 524288 x 64 120 and 108, 131072 x 1000 330 and 287.
 template <typename T, int MODE, int LANES, int NV>
 __global__ void __launch_bounds__(256, MODE == LG_POLICY ? 4 : 1)
 short_kernel(Rows R, Policy P, Outs O) {

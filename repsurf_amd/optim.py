@@ -373,7 +373,8 @@ class AdamW(Adam):
             if any(g.layout is not torch.strided for g in some):
                 raise _lib.RepSurfHipError("repsurf_amd.optim.AdamW: gradients must be dense and of their parameter's type")
             at = list(map(_address, some)) + [g is None for g in grads]
-        plan = (list(map(_address, params)), list(map(_size, params)), list(map(_type, params)), at, list(map(_type, some)))      # (a gradient has its parameter's shape)
+        # (a gradient has its parameter's shape)
+        plan = (list(map(_address, params)), list(map(_size, params)), list(map(_type, params)), at, list(map(_type, some)))
         if plan == st["plan"] and all(map(_dense, some)) and all(map(_dense, params)):
             return st["tables"], None
         rows, keep, seen = ([], []), [], set()
